@@ -70,6 +70,13 @@ SIGNATURES = {
     "nvn_dp_recv_bytes": (_sz, [_i64, _int]),
     "nvn_ln_bwd_dp": (_int, [_int, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _sz,
                              _c.POINTER(DpComm), _vp]),
+    "nvn_ln_bwd_residual_workspace_bytes": (_sz, [_int, _i64, _i64]),
+    "nvn_ln_bwd_residual": (_int, [_int, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _sz,
+                                   _vp]),
+    "nvn_rms_fwd": (_int, [_int, _vp, _vp, _i64, _i64, _c.c_float, _vp, _vp, _vp]),
+    "nvn_rms_fwd_residual": (_int, [_int, _vp, _vp, _vp, _i64, _i64, _c.c_float, _vp, _vp, _vp, _vp]),
+    "nvn_rms_bwd_workspace_bytes": (_sz, [_int, _i64, _i64]),
+    "nvn_rms_bwd": (_int, [_int, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _sz, _vp]),
     "nvn_ln_bwd_noalloc": (_int, [_int, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp]),
     "nvn_in_bwd_dp": (_int, [_int, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _vp, _vp, _vp,
                              _vp, _sz, _c.POINTER(DpComm), _vp]),

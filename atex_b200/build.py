@@ -37,6 +37,8 @@ def _units():
     for t, tname in ((0, "f32"), (1, "f16"), (2, "bf16")):
         for b, dname in ((0, "fwd"), (1, "bwd")):
             units.append((f"rows_{tname}_{dname}.o", "rows_inst.cu", [f"-DNVN_T={t}", f"-DNVN_BWD={b}"]))
+            units.append((f"rows_rms_{tname}_{dname}.o", "rows_rms_inst.cu",
+                          [f"-DNVN_T={t}", f"-DNVN_BWD={b}"]))
         units.append((f"rows_res_{tname}.o", "rows_res_inst.cu", [f"-DNVN_T={t}"]))
     units.append(("rows_wide.o", "rows_wide.cu", []))
     units.append(("twophase.o", "twophase.cu", []))
@@ -46,6 +48,8 @@ def _units():
     units.append(("nlc_small.o", "nlc_small.cu", []))
     units.append(("nlc_stream.o", "nlc_stream.cu", []))
     units.append(("nvnorms_api.o", "nvnorms_api.cu", []))
+    units.append(("rows_generic.o", "rows_generic.cu", []))
+    units.append(("rms_api.o", "rms_api.cu", []))
     units.append(("noalloc.o", "noalloc.cu", []))
     return units
 

@@ -4,7 +4,9 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <atomic>
+#include <initializer_list>
 
 struct nvn_dp_comm;
 
@@ -127,6 +129,39 @@ inline cudaLaunchConfig_t dependent_launch_config(dim3 grid, dim3 block, size_t 
   return cfg;
 }
 
+// Remembers `e` for nvn_last_cuda_error() and clears it; returns NVN_ERR_CUDA.
+int fail_cuda(cudaError_t e);
+
+inline bool aligned(const void* p, size_t a) {
+  return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0;
+}
+inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
+// codes of nvn_dtype: 0 = float, 1 = half, 2 = bfloat16
+inline size_t dtype_size(int dtype) { return dtype == 0 ? 4 : 2; }
+inline int full_epv(int dtype) { return dtype == 0 ? 4 : 8; }
+inline bool valid_dtype(int d) { return d >= 0 && d <= 2; }
+
+// Largest power-of-two alignment (capped at 16) shared by all the pointers given.
+inline size_t common_alignment(std::initializer_list<const void*> ptrs) {
+  uintptr_t bits = 0;
+  for (const void* p : ptrs) bits |= reinterpret_cast<uintptr_t>(p);
+  size_t a = 16;
+  while (a > 1 && (bits & (a - 1)) != 0) a >>= 1;
+  return a;
+}
+
+// Elements per access for rows of width D: the widest of (full, full/2, full/4) that
+// divides D and fits the alignment, else single elements.
+// `align` is the activations' alignment, `par_align` that of the fp32 parameters, which are
+// read e floats at a time in accesses of at most 16 bytes.
+inline int pick_epv(int dtype, int64_t D, size_t align, size_t par_align) {
+  const int V = full_epv(dtype);
+  const size_t es = dtype_size(dtype);
+  for (int e = V; e >= 2; e >>= 1)
+    if (D % e == 0 && e * es <= align && std::min<size_t>(16, e * 4) <= par_align) return e;
+  return 1;
+}
+
 int device_sm_count();
 void count_launch();
 // Whether the row kernels are launched with the programmatic-stream-serialization
@@ -245,6 +280,41 @@ cudaError_t residual_add_bf16(const void* x, const void* res, void* out, int64_t
 // The fallback's element-wise s = T(x + res) for any size and alignment.
 cudaError_t residual_add_launch(int dtype, const void* x, const void* res, void* sum_out,
                                 int64_t count, cudaStream_t s);
+
+// RMS normalisation and the residual norms' gradients (rows_rms_inst.cu), one entry point per
+// (dtype, direction).  `form`: forward 0 = RMS, 1 = RMS of s = T(x + res); backward 0 = RMS,
+// 1 = RMS with the residual branch's gradient (a.res) added to dx, 2 = LayerNorm with it.
+// `shape` indexes the same tables as the LayerNorm kernels (entries with CS == 1 only).  RMS
+// reads no mean and no beta; its partial rows are [D] instead of [2][D].
+#define NVN_DECLARE_ROWS_RMS(NAME)                                                      \
+  cudaError_t NAME(int form, int epv, int shape, const RowsResArgs& a, cudaStream_t s, \
+                   bool dry_run, RowsPlan* plan);
+NVN_DECLARE_ROWS_RMS(rows_rms_f32_fwd)
+NVN_DECLARE_ROWS_RMS(rows_rms_f32_bwd)
+NVN_DECLARE_ROWS_RMS(rows_rms_f16_fwd)
+NVN_DECLARE_ROWS_RMS(rows_rms_f16_bwd)
+NVN_DECLARE_ROWS_RMS(rows_rms_bf16_fwd)
+NVN_DECLARE_ROWS_RMS(rows_rms_bf16_bwd)
+
+// The same operators for any row width (rows_generic.cu): `vec` = 128-bit accesses, else
+// single elements.  a.res may be null (no residual).  Backward: `coef` holds [N][rms ? 1 : 2]
+// floats of scratch and a.ws `slices` partial rows (generic_slices).
+int generic_slices(int64_t N, int64_t D, int epv);
+cudaError_t generic_launch(int dtype, bool vec, bool bwd, bool rms, const RowsResArgs& a,
+                           float* coef, int slices, cudaStream_t s);
+
+// out[c] = sum over `rows` partial rows of `cols` floats, in a fixed order; one or two
+// segments of the same width in one launch (launched as a dependent of the kernel before it).
+struct ColsumSegment {
+  const float* partials;
+  float* out;
+  int64_t rows;
+};
+struct ColsumArgs {
+  ColsumSegment seg[2];
+  int64_t cols;
+};
+cudaError_t colsum_launch(const ColsumArgs& a, int segments, cudaStream_t s);
 
 // Deterministic second stage of the dgamma / dbeta reduction: sums P partial
 // rows of [2][F] floats (dgamma then dbeta) in a fixed order.

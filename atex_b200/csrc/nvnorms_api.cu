@@ -124,10 +124,6 @@ int pick_shape(const Shape* table, int n, int64_t nvec, int64_t tensor_bytes, in
   return best;
 }
 
-inline bool aligned(const void* p, size_t a) {
-  return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0;
-}
-inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 // Scratch the column reduction may use to split very many partial rows of F features into
 // slabs (colreduce.cu); only InstanceNorm over thousands of items gets there.
 inline size_t colreduce_scratch_bytes(int64_t partial_rows, int64_t F) {
@@ -135,31 +131,9 @@ inline size_t colreduce_scratch_bytes(int64_t partial_rows, int64_t F) {
              ? align_up(static_cast<size_t>(kColreduceScratchRows) * 2 * F * 4, 256)
              : 0;
 }
-inline size_t dtype_size(int dtype) { return dtype == NVN_F32 ? 4 : 2; }
-inline int full_epv(int dtype) { return dtype == NVN_F32 ? 4 : 8; }
 
 typedef cudaError_t (*RowsFn)(bool, int, int, const RowsArgs&, cudaStream_t, bool, RowsPlan*);
 
-// Largest power-of-two alignment (capped at 16) shared by all the pointers given.
-inline size_t common_alignment(std::initializer_list<const void*> ptrs) {
-  uintptr_t bits = 0;
-  for (const void* p : ptrs) bits |= reinterpret_cast<uintptr_t>(p);
-  size_t a = 16;
-  while (a > 1 && (bits & (a - 1)) != 0) a >>= 1;
-  return a;
-}
-
-// Elements per access for rows of width D: the widest of (full, full/2, full/4) that
-// divides D and fits the alignment, else single elements.
-// `align` is the activations' alignment, `par_align` that of the fp32 parameters, which are
-// read e floats at a time in accesses of at most 16 bytes.
-inline int pick_epv(int dtype, int64_t D, size_t align, size_t par_align) {
-  const int V = full_epv(dtype);
-  const size_t es = dtype_size(dtype);
-  for (int e = V; e >= 2; e >>= 1)
-    if (D % e == 0 && e * es <= align && std::min<size_t>(16, e * 4) <= par_align) return e;
-  return 1;
-}
 RowsFn rows_fn(int dtype, bool bwd) {
   switch (dtype) {
     case NVN_F32:
@@ -169,12 +143,6 @@ RowsFn rows_fn(int dtype, bool bwd) {
     default:
       return bwd ? rows_bf16_bwd : rows_bf16_fwd;
   }
-}
-
-int fail_cuda(cudaError_t e) {
-  t_last_cuda_error = static_cast<int>(e);
-  (void)cudaGetLastError();
-  return NVN_ERR_CUDA;
 }
 
 // ---------------------------------------------------------------------------
@@ -674,9 +642,13 @@ int zero_grads(float* dgamma, float* dbeta, int64_t F, cudaStream_t stream) {
   return e == cudaSuccess ? NVN_OK : fail_cuda(e);
 }
 
-inline bool valid_dtype(int d) { return d == NVN_F32 || d == NVN_F16 || d == NVN_BF16; }
-
 }  // namespace
+
+int fail_cuda(cudaError_t e) {
+  t_last_cuda_error = static_cast<int>(e);
+  (void)cudaGetLastError();
+  return NVN_ERR_CUDA;
+}
 
 int device_sm_count() {
   int v = g_sm_count.load(std::memory_order_relaxed);

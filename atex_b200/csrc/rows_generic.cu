@@ -1,0 +1,285 @@
+// RMS normalisation and residual norm gradients for rows that the row-cached kernels of
+// rows_rms_inst.cu do not hold (wider than a CTA's registers, or wide and of a width that
+// rules out vector accesses), and the column sum that ends their gradients.
+//
+//   forward    one CTA per row: pass 1 sums the squares (and writes s = T(x + res)), pass 2
+//              reads the row again - from L2 - and writes y.
+//   backward   rms_rowsum_kernel: one CTA per row, the row's mean(gy xh) (and mean(gy) for
+//              LayerNorm);  rms_columns_kernel: a thread owns EPV columns of a slice of rows,
+//              writes dx and keeps dgamma (dbeta) of its columns in registers;  the partial
+//              rows of the slices are summed by colsum_kernel in a fixed order.
+//
+// Bound by HBM: the second pass over x (and dy) misses L2 once a tensor is far larger than
+// it, so forward moves up to 3 tensor passes for 2 counted, backward 5 for 3.
+#include "nvn_common.cuh"
+#include "nvn_host.h"
+
+namespace nvn {
+
+namespace {
+
+constexpr int kRowBlock = 512;
+constexpr int kColBlock = 128;
+
+template <typename T, int EPV, bool RES>
+__global__ void __launch_bounds__(kRowBlock) rms_generic_fwd_kernel(const RowsResArgs a) {
+  using M = typename MathSel<EPV>::M;
+  using E = typename M::E;
+  constexpr int NE = MathSel<EPV>::NE;
+  using P = Pack<T, EPV>;
+  __shared__ ReduceSmem<1, kRowBlock> sm;
+  int phase = 0;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t rowvecs = a.D / EPV;
+  const float inv_D = 1.0f / static_cast<float>(a.D);
+  for (int64_t row = blockIdx.x; row < a.N; row += gridDim.x) {
+    const P* xp = reinterpret_cast<const P*>(a.x) + row * rowvecs;
+    const P* rp = reinterpret_cast<const P*>(a.res) + (RES ? row * rowvecs : 0);
+    P* sp = reinterpret_cast<P*>(a.sum_out) + (RES ? row * rowvecs : 0);
+    P* yp = reinterpret_cast<P*>(a.out) + row * rowvecs;
+    E acc = M::bcast(0.f);
+    for (int64_t i = tid; i < rowvecs; i += kRowBlock) {
+      E v[NE];
+      unpack<T, EPV>(load_keep<T, EPV>(reinterpret_cast<const T*>(xp + i)), v);
+      if constexpr (RES) {
+        E r[NE];
+        unpack<T, EPV>(load_keep<T, EPV>(reinterpret_cast<const T*>(rp + i)), r);
+#pragma unroll
+        for (int e = 0; e < NE; ++e) v[e] = M::add(v[e], r[e]);
+        const P s = repack<T, EPV>(v);
+        sp[i] = s;
+        unpack<T, EPV>(s, v);
+      }
+#pragma unroll
+      for (int e = 0; e < NE; ++e) acc = M::fma(v[e], v[e], acc);
+    }
+    float q[1] = {M::hsum(acc) * inv_D};  // the thread's share of the mean: see rows_fwd_kernel
+    group_allreduce<1, kRowBlock, kRowBlock, 1>(q, sm, phase, warp, lane);
+    const float inv = rsqrtf(q[0] + a.eps);
+    const E iv2 = M::bcast(inv);
+    // the thread reads back only what it wrote itself (s), or what nobody has written (x)
+    const P* back = RES ? sp : xp;
+    for (int64_t i = tid; i < rowvecs; i += kRowBlock) {
+      E v[NE], g[NE];
+      unpack<T, EPV>(load_keep<T, EPV>(reinterpret_cast<const T*>(back + i)), v);
+      load_param_lanes<EPV>(a.gamma, i * EPV, g);
+#pragma unroll
+      for (int e = 0; e < NE; ++e) v[e] = M::mul(M::mul(v[e], iv2), g[e]);
+      yp[i] = repack<T, EPV>(v);
+    }
+    if (tid == 0 && a.ivar != nullptr) a.ivar[row] = inv;
+  }
+}
+
+// coef[row][NR]: mean(gy) (LayerNorm only), mean(gy xh)
+template <typename T, int EPV, bool RMS>
+__global__ void __launch_bounds__(kRowBlock) rms_rowsum_kernel(const RowsResArgs a, float* coef) {
+  using M = typename MathSel<EPV>::M;
+  using E = typename M::E;
+  constexpr int NE = MathSel<EPV>::NE;
+  constexpr int NR = RMS ? 1 : 2;
+  using P = Pack<T, EPV>;
+  __shared__ ReduceSmem<NR, kRowBlock> sm;
+  int phase = 0;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t rowvecs = a.D / EPV;
+  const float inv_D = 1.0f / static_cast<float>(a.D);
+  for (int64_t row = blockIdx.x; row < a.N; row += gridDim.x) {
+    const P* xp = reinterpret_cast<const P*>(a.x) + row * rowvecs;
+    const P* dyp = reinterpret_cast<const P*>(a.dy) + row * rowvecs;
+    const E nm = M::bcast(RMS ? 0.f : -a.mean_in[row]);
+    const E iv2 = M::bcast(a.ivar_in[row]);
+    E r0 = M::bcast(0.f), r1 = M::bcast(0.f);
+    for (int64_t i = tid; i < rowvecs; i += kRowBlock) {
+      E v[NE], d[NE], g[NE];
+      unpack<T, EPV>(load_keep<T, EPV>(reinterpret_cast<const T*>(xp + i)), v);
+      unpack<T, EPV>(load_keep<T, EPV>(reinterpret_cast<const T*>(dyp + i)), d);
+      load_param_lanes<EPV>(a.gamma, i * EPV, g);
+#pragma unroll
+      for (int e = 0; e < NE; ++e) {
+        d[e] = M::mul(d[e], g[e]);
+        if constexpr (!RMS) r0 = M::add(r0, d[e]);
+        r1 = M::fma(d[e], M::mul(RMS ? v[e] : M::add(v[e], nm), iv2), r1);
+      }
+    }
+    float red[NR];
+    if constexpr (!RMS) red[0] = M::hsum(r0);
+    red[NR - 1] = M::hsum(r1);
+    group_allreduce<NR, kRowBlock, kRowBlock, 1>(red, sm, phase, warp, lane);
+    if (tid == 0) {
+#pragma unroll
+      for (int k = 0; k < NR; ++k) coef[row * NR + k] = red[k] * inv_D;
+    }
+  }
+}
+
+// a.ws: partial rows [gridDim.y][NR][D]
+template <typename T, int EPV, bool RMS>
+__global__ void __launch_bounds__(kColBlock)
+    rms_columns_kernel(const RowsResArgs a, const float* __restrict__ coef, int64_t rows_per_slice) {
+  using M = typename MathSel<EPV>::M;
+  using E = typename M::E;
+  constexpr int NE = MathSel<EPV>::NE;
+  constexpr int NR = RMS ? 1 : 2;
+  using P = Pack<T, EPV>;
+  const int64_t rowvecs = a.D / EPV;
+  const int64_t vec = static_cast<int64_t>(blockIdx.x) * kColBlock + threadIdx.x;
+  if (vec >= rowvecs) return;
+  const int64_t r_begin = static_cast<int64_t>(blockIdx.y) * rows_per_slice;
+  const int64_t r_end = r_begin + rows_per_slice < a.N ? r_begin + rows_per_slice : a.N;
+  const P* xp = reinterpret_cast<const P*>(a.x) + vec;
+  const P* dyp = reinterpret_cast<const P*>(a.dy) + vec;
+  const P* dsp = reinterpret_cast<const P*>(a.res) + vec;
+  const bool third = a.res != nullptr;
+  P* op = reinterpret_cast<P*>(a.out) + vec;
+  E g[NE], dg[NE], db[NE];
+  load_param_lanes<EPV>(a.gamma, vec * EPV, g);
+#pragma unroll
+  for (int e = 0; e < NE; ++e) dg[e] = db[e] = M::bcast(0.f);
+  constexpr int U = 4;   // rows in flight per thread
+  for (int64_t r0 = r_begin; r0 < r_end; r0 += U) {
+    P px[U], pd[U], ps[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (r0 + u < r_end) {
+        px[u] = load_stream<T, EPV>(reinterpret_cast<const T*>(xp + (r0 + u) * rowvecs), 0);
+        pd[u] = load_stream<T, EPV>(reinterpret_cast<const T*>(dyp + (r0 + u) * rowvecs), 0);
+        if (third) ps[u] = load_stream<T, EPV>(reinterpret_cast<const T*>(dsp + (r0 + u) * rowvecs), 0);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t row = r0 + u;
+      if (row < r_end) {
+        E v[NE], d[NE];
+        unpack<T, EPV>(px[u], v);
+        unpack<T, EPV>(pd[u], d);
+        const float iv = __ldg(a.ivar_in + row);
+        const E iv2 = M::bcast(iv);
+        const E nm = M::bcast(RMS ? 0.f : -__ldg(a.mean_in + row));
+        const E nm0 = M::bcast(RMS ? 0.f : -__ldg(coef + row * NR));
+        const E nm1 = M::bcast(-__ldg(coef + row * NR + NR - 1));
+#pragma unroll
+        for (int e = 0; e < NE; ++e) {
+          v[e] = M::mul(RMS ? v[e] : M::add(v[e], nm), iv2);
+          dg[e] = M::fma(d[e], v[e], dg[e]);
+          if constexpr (!RMS) db[e] = M::add(db[e], d[e]);
+          d[e] = M::mul(d[e], g[e]);
+          v[e] = RMS ? M::fma(v[e], nm1, d[e]) : M::add(d[e], M::fma(v[e], nm1, nm0));
+        }
+        if (third) {
+          E s[NE];
+          unpack<T, EPV>(ps[u], s);
+#pragma unroll
+          for (int e = 0; e < NE; ++e) v[e] = M::fma(v[e], iv2, s[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < NE; ++e) v[e] = M::mul(v[e], iv2);
+        }
+        store_stream<T, EPV>(reinterpret_cast<T*>(op + row * rowvecs), 0, repack<T, EPV>(v));
+      }
+    }
+  }
+  float* w = a.ws + static_cast<int64_t>(blockIdx.y) * NR * a.D;
+  store_param_lanes<EPV>(w, vec * EPV, dg);
+  if constexpr (!RMS) store_param_lanes<EPV>(w + a.D, vec * EPV, db);
+}
+
+template <typename T, int EPV>
+cudaError_t fwd_t(const RowsResArgs& a, cudaStream_t s) {
+  const int64_t most = static_cast<int64_t>(device_sm_count()) * 4;  // 4 CTAs of 512 threads fill an SM
+  const unsigned grid = static_cast<unsigned>(a.N < most ? a.N : most);
+  count_launch();
+  if (a.res != nullptr) {
+    rms_generic_fwd_kernel<T, EPV, true><<<grid, kRowBlock, 0, s>>>(a);
+  } else {
+    rms_generic_fwd_kernel<T, EPV, false><<<grid, kRowBlock, 0, s>>>(a);
+  }
+  return cudaGetLastError();
+}
+
+template <typename T, int EPV, bool RMS>
+cudaError_t bwd_t(const RowsResArgs& a, float* coef, int slices, cudaStream_t s) {
+  const int64_t most = static_cast<int64_t>(device_sm_count()) * 4;
+  count_launch();
+  rms_rowsum_kernel<T, EPV, RMS>
+      <<<static_cast<unsigned>(a.N < most ? a.N : most), kRowBlock, 0, s>>>(a, coef);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  const int64_t tiles = (a.D / EPV + kColBlock - 1) / kColBlock;
+  count_launch();
+  rms_columns_kernel<T, EPV, RMS>
+      <<<dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(slices)), kColBlock, 0, s>>>(
+          a, coef, (a.N + slices - 1) / slices);
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t generic_t(bool vec, bool bwd, bool rms, const RowsResArgs& a, float* coef, int slices,
+                      cudaStream_t s) {
+  constexpr int V = VecTraits<T>::kFull;
+  if (!bwd) return vec ? fwd_t<T, V>(a, s) : fwd_t<T, 1>(a, s);
+  if (rms) return vec ? bwd_t<T, V, true>(a, coef, slices, s) : bwd_t<T, 1, true>(a, coef, slices, s);
+  return vec ? bwd_t<T, V, false>(a, coef, slices, s) : bwd_t<T, 1, false>(a, coef, slices, s);
+}
+
+// ---- column sum ---------------------------------------------------------------
+// Block (32, TY): thread (tx, ty) adds rows ty, ty + TY, ... of column tx in increasing order,
+// then the TY sums are added in increasing ty: a fixed order, the same bits on every run.
+constexpr int kSumX = 32;
+
+template <int TY>
+__global__ void __launch_bounds__(kSumX* TY) colsum_kernel(const ColsumArgs a) {
+  __shared__ float tile[TY][kSumX + 1];
+  const int tx = threadIdx.x, ty = threadIdx.y;
+  const ColsumSegment seg = blockIdx.y == 0 ? a.seg[0] : a.seg[1];
+  const int64_t col = static_cast<int64_t>(blockIdx.x) * kSumX + tx;
+  griddep_launch_dependents();
+  griddep_wait();  // the partial rows come from the kernel launched just before
+  float s = 0.f;
+  if (col < a.cols) {
+    for (int64_t p = ty; p < seg.rows; p += TY) s += seg.partials[p * a.cols + col];
+  }
+  tile[ty][tx] = s;
+  __syncthreads();
+  if (ty == 0 && col < a.cols) {
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < TY; ++k) t += tile[k][tx];
+    seg.out[col] = t;
+  }
+}
+
+template <int TY>
+cudaError_t colsum_t(const ColsumArgs& a, int segments, cudaStream_t s) {
+  cudaLaunchAttribute attr;
+  const cudaLaunchConfig_t cfg = dependent_launch_config(
+      dim3(static_cast<unsigned>((a.cols + kSumX - 1) / kSumX), static_cast<unsigned>(segments)),
+      dim3(kSumX, TY), 0, s, &attr);
+  count_launch();
+  return cudaLaunchKernelEx(&cfg, colsum_kernel<TY>, a);
+}
+
+}  // namespace
+
+int generic_slices(int64_t N, int64_t D, int epv) {
+  // enough (column tile, slice) CTAs for eight per SM, at least eight rows in a slice
+  const int64_t tiles = (D / epv + kColBlock - 1) / kColBlock;
+  int64_t n = static_cast<int64_t>(device_sm_count()) * 8 / tiles;
+  if (n > (N + 7) / 8) n = (N + 7) / 8;
+  return static_cast<int>(n < 1 ? 1 : n);
+}
+
+cudaError_t generic_launch(int dtype, bool vec, bool bwd, bool rms, const RowsResArgs& a,
+                           float* coef, int slices, cudaStream_t s) {
+  if (dtype == 0) return generic_t<float>(vec, bwd, rms, a, coef, slices, s);
+  if (dtype == 1) return generic_t<__half>(vec, bwd, rms, a, coef, slices, s);
+  return generic_t<__nv_bfloat16>(vec, bwd, rms, a, coef, slices, s);
+}
+
+cudaError_t colsum_launch(const ColsumArgs& a, int segments, cudaStream_t s) {
+  const int64_t rows = segments > 1 && a.seg[1].rows > a.seg[0].rows ? a.seg[1].rows : a.seg[0].rows;
+  return rows <= 32 ? colsum_t<4>(a, segments, s) : colsum_t<32>(a, segments, s);
+}
+
+}  // namespace nvn

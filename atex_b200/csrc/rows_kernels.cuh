@@ -130,7 +130,7 @@ struct RowRing {
 
   // Called by one thread: start the copies of the batch whose first row is `row_first`
   // (the CTA's batch base, without the row-group offset) into stage `s`.
-  __device__ __forceinline__ void issue(int s, const T* const (&src)[NT], int64_t row_first,
+  __device__ __forceinline__ void issue(int s, const T* const* src, int64_t row_first,
                                         int64_t N, int64_t D, unsigned crank) {
     unsigned char* dst = base + static_cast<size_t>(s) * stage_bytes;
     if constexpr (CS == 1) {
@@ -225,9 +225,11 @@ __device__ __forceinline__ void ring_give_up(Ring& ring, int* status, int64_t j,
 // forward
 // ---------------------------------------------------------------------------
 //   RES   (forward only) the row that is normalised is s = T(x + res); s is written to
-//         a.sum_out.  Plain or register-prefetch loads only.
+//         a.sum_out.  In a ring, x and res sit in the same stage.
+//   RMS   root mean square: no mean, no beta; one reduction instead of two, and a.ivar is
+//         1/sqrt(mean(x^2) + eps) (not written when a.ivar is null).
 template <typename T, int EPV, int TPR, int VPT, int CS, int RB, bool PR, int MINB, int PF,
-          bool EXACT, bool ROW_AFFINE, bool RES = false>
+          bool EXACT, bool ROW_AFFINE, bool RES = false, bool RMS = false>
 __global__ void __launch_bounds__(RowBlock<TPR, MINB>::kBlock)
     rows_fwd_kernel(const typename std::conditional<RES, RowsResArgs, RowsArgs>::type a) {
   constexpr int BLOCK = RowBlock<TPR, MINB>::kBlock;
@@ -238,7 +240,8 @@ __global__ void __launch_bounds__(RowBlock<TPR, MINB>::kBlock)
   constexpr int VSTRIDE = Map::kStride;
   static_assert(CS == 1 || RPC == 1, "cluster kernels own one row per cluster");
   static_assert(!(TMA && CS > 1) || EXACT, "cluster slices need rows that fill the shape");
-  static_assert(!RES || (!TMA && CS == 1 && !ROW_AFFINE), "residual add: LayerNorm, one CTA per row, no ring");
+  static_assert(!RES || (CS == 1 && !ROW_AFFINE), "residual add: contiguous rows, one CTA per row");
+  static_assert(!RMS || (CS == 1 && !ROW_AFFINE), "root mean square: contiguous rows, one CTA per row");
   constexpr bool PARAMS_IN_REGS = !ROW_AFFINE && PR;
   using M = typename MathSel<EPV>::M;
   using E = typename M::E;
@@ -300,7 +303,8 @@ __global__ void __launch_bounds__(RowBlock<TPR, MINB>::kBlock)
     for (int v = 0; v < VPT; ++v) {
       if (EXACT || v < nvalid) {
         load_param_lanes<EPV>(a.gamma, static_cast<int64_t>(vec0 + v * VSTRIDE) * EPV, g[v]);
-        load_param_lanes<EPV>(a.beta, static_cast<int64_t>(vec0 + v * VSTRIDE) * EPV, b[v]);
+        if constexpr (!RMS)
+          load_param_lanes<EPV>(a.beta, static_cast<int64_t>(vec0 + v * VSTRIDE) * EPV, b[v]);
       } else {
 #pragma unroll
         for (int e = 0; e < NE; ++e) g[v][e] = b[v][e] = M::bcast(0.f);
@@ -313,14 +317,18 @@ __global__ void __launch_bounds__(RowBlock<TPR, MINB>::kBlock)
   const int64_t nb = batch0 < N ? (N - batch0 + stride - 1) / stride : 0;
   RowTile<T, EPV, VPT, RB> tile;
   RowTile<T, EPV, VPT, RES ? RB : 1> rtile;   // the residual's row batch
-  RowRing<T, EPV, VPT, RB, RPC, CS, STAGES, 1> ring;
-  const T* const srcs[1] = {static_cast<const T*>(a.x)};
-  unsigned roff[RB];
+  RowRing<T, EPV, VPT, RB, RPC, CS, STAGES, RES ? 2 : 1> ring;
+  const T* srcs[RES ? 2 : 1];
+  srcs[0] = static_cast<const T*>(a.x);
+  if constexpr (RES) srcs[1] = static_cast<const T*>(a.res);
+  unsigned roff[RB], rroff[RES ? RB : 1];
   if constexpr (TMA) {
     ring.init(ring_mem, ring_bars, D);
 #pragma unroll
-    for (int r = 0; r < RB; ++r)
+    for (int r = 0; r < RB; ++r) {
       roff[r] = ring.thread_offset(0, CS == 1 ? r * RPC + group : r, lir);
+      if constexpr (RES) rroff[r] = ring.thread_offset(1, r * RPC + group, lir);
+    }
     if (tid == 0) {
       for (int64_t k = 0; k < STAGES && k < nb; ++k)
         ring.issue(static_cast<int>(k), srcs, batch0 + k * stride, N, D, crank);
@@ -336,6 +344,8 @@ __global__ void __launch_bounds__(RowBlock<TPR, MINB>::kBlock)
       const int s = static_cast<int>(j % STAGES);
       const bool ok = ring.wait(s, static_cast<unsigned>(j / STAGES));
       ring_tile<T, EPV, VPT, RB, RPC, TPR, EXACT>(ring.stage_ptr(s), roff, row0, N, nvalid, tile);
+      if constexpr (RES)
+        ring_tile<T, EPV, VPT, RB, RPC, TPR, EXACT>(ring.stage_ptr(s), rroff, row0, N, nvalid, rtile);
       // every thread has its copy of the stage: it can be refilled
       if (__syncthreads_or(!ok) && !ring.dead) ring_give_up<decltype(ring), STAGES>(ring, a.status, j, nb);
       if (tid == 0 && !ring.dead && j + STAGES < nb)
@@ -367,9 +377,12 @@ __global__ void __launch_bounds__(RowBlock<TPR, MINB>::kBlock)
           unpack<T, EPV>(sp, xv[r][v]);
         }
 #pragma unroll
-        for (int e = 0; e < NE; ++e) acc = M::add(acc, xv[r][v][e]);
+        for (int e = 0; e < NE; ++e)
+          acc = RMS ? M::fma(xv[r][v][e], xv[r][v][e], acc) : M::add(acc, xv[r][v][e]);
       }
-      s_[r] = M::hsum(acc);
+      // (RMS: the thread's share of the mean, so that a row whose mean square fits in fp32 does
+      // not overflow in the sum over its threads)
+      s_[r] = RMS ? M::hsum(acc) * inv_D : M::hsum(acc);
     }
     if constexpr (PF == 1) {
       load_tile<T, EPV, VPT, RB, RPC, VSTRIDE, EXACT>(xp, row0 + stride, N, rowvecs, nvalid, tile);
@@ -379,29 +392,34 @@ __global__ void __launch_bounds__(RowBlock<TPR, MINB>::kBlock)
     group_allreduce<RB, TPR, BLOCK, CS>(s_, sm, phase, warp, lane);
 
     float mean[RB], q[RB];
+    if constexpr (RMS) {
 #pragma unroll
-    for (int r = 0; r < RB; ++r) {
-      mean[r] = s_[r] * inv_D;
-      const E nm = M::bcast(-mean[r]);
-      E acc = M::bcast(0.f);
+      for (int r = 0; r < RB; ++r) q[r] = s_[r];
+    } else {
 #pragma unroll
-      for (int v = 0; v < VPT; ++v) {
-        if (EXACT || v < nvalid) {
+      for (int r = 0; r < RB; ++r) {
+        mean[r] = s_[r] * inv_D;
+        const E nm = M::bcast(-mean[r]);
+        E acc = M::bcast(0.f);
 #pragma unroll
-          for (int e = 0; e < NE; ++e) {
-            xv[r][v][e] = M::add(xv[r][v][e], nm);  // centred value, reused below
-            acc = M::fma(xv[r][v][e], xv[r][v][e], acc);
+        for (int v = 0; v < VPT; ++v) {
+          if (EXACT || v < nvalid) {
+#pragma unroll
+            for (int e = 0; e < NE; ++e) {
+              xv[r][v][e] = M::add(xv[r][v][e], nm);  // centred value, reused below
+              acc = M::fma(xv[r][v][e], xv[r][v][e], acc);
+            }
           }
         }
+        q[r] = M::hsum(acc);
       }
-      q[r] = M::hsum(acc);
+      group_allreduce<RB, TPR, BLOCK, CS>(q, sm, phase, warp, lane);
     }
-    group_allreduce<RB, TPR, BLOCK, CS>(q, sm, phase, warp, lane);
 
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
       const int64_t row = row0 + r * RPC;
-      const float ivar = rsqrtf(fmaf(q[r], inv_D, eps));
+      const float ivar = rsqrtf(RMS ? q[r] + eps : fmaf(q[r], inv_D, eps));
       if (row < N) {
         float gr = 1.f, br = 0.f;
         if constexpr (ROW_AFFINE) {
@@ -423,20 +441,28 @@ __global__ void __launch_bounds__(RowBlock<TPR, MINB>::kBlock)
             } else if constexpr (PARAMS_IN_REGS) {
 #pragma unroll
               for (int e = 0; e < NE; ++e)
-                o[e] = M::fma(M::mul(xv[r][v][e], iv2), g[v][e], b[v][e]);
+                o[e] = RMS ? M::mul(M::mul(xv[r][v][e], iv2), g[v][e])
+                           : M::fma(M::mul(xv[r][v][e], iv2), g[v][e], b[v][e]);
             } else {
               E gg[NE], bb[NE];
               load_param_lanes<EPV>(a.gamma, static_cast<int64_t>(vec0 + v * VSTRIDE) * EPV, gg);
-              load_param_lanes<EPV>(a.beta, static_cast<int64_t>(vec0 + v * VSTRIDE) * EPV, bb);
+              if constexpr (!RMS)
+                load_param_lanes<EPV>(a.beta, static_cast<int64_t>(vec0 + v * VSTRIDE) * EPV, bb);
 #pragma unroll
-              for (int e = 0; e < NE; ++e) o[e] = M::fma(M::mul(xv[r][v][e], iv2), gg[e], bb[e]);
+              for (int e = 0; e < NE; ++e)
+                o[e] = RMS ? M::mul(M::mul(xv[r][v][e], iv2), gg[e])
+                           : M::fma(M::mul(xv[r][v][e], iv2), gg[e], bb[e]);
             }
             store_stream<T, EPV>(reinterpret_cast<T*>(rp + v * VSTRIDE), 0, repack<T, EPV>(o));
           }
         }
         if (lir == 0 && crank == 0) {
-          a.mean[row] = mean[r];
-          a.ivar[row] = ivar;
+          if constexpr (RMS) {
+            if (a.ivar != nullptr) a.ivar[row] = ivar;
+          } else {
+            a.mean[row] = mean[r];
+            a.ivar[row] = ivar;
+          }
         }
       }
     }
@@ -448,10 +474,14 @@ __global__ void __launch_bounds__(RowBlock<TPR, MINB>::kBlock)
 // ---------------------------------------------------------------------------
 // backward
 // ---------------------------------------------------------------------------
+//   RMS   root mean square: x-hat = x * ivar, no mean, one sum per row and no dbeta; a
+//         partial row in the workspace is [D] instead of [2][D].
+//   DRES  the gradient that reaches the normalised row from the residual branch (a.res) is
+//         added to dx before its one rounding: a third tensor beside x and dy.
 template <typename T, int EPV, int TPR, int VPT, int CS, int RB, bool PR, int MINB, int PF,
-          bool EXACT, bool ROW_AFFINE>
+          bool EXACT, bool ROW_AFFINE, bool RMS = false, bool DRES = false>
 __global__ void __launch_bounds__(RowBlock<TPR, MINB>::kBlock)
-    rows_bwd_kernel(const RowsArgs a) {
+    rows_bwd_kernel(const typename std::conditional<DRES, RowsResArgs, RowsArgs>::type a) {
   constexpr int BLOCK = RowBlock<TPR, MINB>::kBlock;
   constexpr int RPC = RowBlock<TPR, MINB>::kRowsPerCta;
   constexpr bool TMA = PF >= 2;
@@ -462,6 +492,8 @@ __global__ void __launch_bounds__(RowBlock<TPR, MINB>::kBlock)
   constexpr int VSTRIDE = Map::kStride;
   static_assert(CS == 1 || RPC == 1, "cluster kernels own one row per cluster");
   static_assert(!(TMA && CS > 1) || EXACT, "cluster slices need rows that fill the shape");
+  static_assert(!(RMS || DRES) || (CS == 1 && !ROW_AFFINE), "contiguous rows, one CTA per row");
+  constexpr int NR = RMS ? 1 : 2;  // sums per row, and [D] vectors per partial row
   constexpr bool PARAMS_IN_REGS = !ROW_AFFINE && PR;
   constexpr int CAP = TPR * VPT * EPV;  // columns one row group covers (CS == 1)
   using M = typename MathSel<EPV>::M;
@@ -476,8 +508,8 @@ __global__ void __launch_bounds__(RowBlock<TPR, MINB>::kBlock)
   griddep_wait();
   extern __shared__ __align__(128) unsigned char ring_mem[];
   __shared__ __align__(8) uint64_t ring_bars[STAGES];
-  __shared__ ReduceSmem<2 * RB, BLOCK> sm;
-  __shared__ float comb[(!ROW_AFFINE && RPC > 1) ? 2 * CAP : 1];
+  __shared__ ReduceSmem<NR * RB, BLOCK> sm;
+  __shared__ float comb[(!ROW_AFFINE && RPC > 1) ? NR * CAP : 1];
   int phase = 0;
 
   const int tid = threadIdx.x;
@@ -508,9 +540,11 @@ __global__ void __launch_bounds__(RowBlock<TPR, MINB>::kBlock)
   const P* __restrict__ xp = reinterpret_cast<const P*>(a.x) + vec0;
   const P* __restrict__ dyp = reinterpret_cast<const P*>(a.dy) + vec0;
   P* __restrict__ dxp = reinterpret_cast<P*>(a.out) + vec0;
+  const P* dsp = nullptr;
+  if constexpr (DRES) dsp = reinterpret_cast<const P*>(a.res) + vec0;
 
   E g[PARAMS_IN_REGS ? VPT : 1][NE];
-  E dg[ROW_AFFINE ? 1 : VPT][NE], db[ROW_AFFINE ? 1 : VPT][NE];
+  E dg[ROW_AFFINE ? 1 : VPT][NE], db[ROW_AFFINE || RMS ? 1 : VPT][NE];
   if constexpr (PARAMS_IN_REGS) {
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
@@ -526,22 +560,30 @@ __global__ void __launch_bounds__(RowBlock<TPR, MINB>::kBlock)
 #pragma unroll
     for (int v = 0; v < VPT; ++v)
 #pragma unroll
-      for (int e = 0; e < NE; ++e) dg[v][e] = db[v][e] = M::bcast(0.f);
+      for (int e = 0; e < NE; ++e) {
+        dg[v][e] = M::bcast(0.f);
+        if constexpr (!RMS) db[v][e] = M::bcast(0.f);
+      }
   }
 
   const int64_t stride = nunits * (RPC * RB);
   const int64_t batch0 = unit * (RPC * RB);
   const int64_t nb = batch0 < N ? (N - batch0 + stride - 1) / stride : 0;
   RowTile<T, EPV, VPT, RB> tx, tdy;
-  RowRing<T, EPV, VPT, RB, RPC, CS, STAGES, 2> ring;
-  const T* const srcs[2] = {static_cast<const T*>(a.x), static_cast<const T*>(a.dy)};
-  unsigned xoff[RB], dyoff[RB];
+  RowTile<T, EPV, VPT, DRES ? RB : 1> tds;  // the residual branch's gradient
+  RowRing<T, EPV, VPT, RB, RPC, CS, STAGES, DRES ? 3 : 2> ring;
+  const T* srcs[DRES ? 3 : 2];
+  srcs[0] = static_cast<const T*>(a.x);
+  srcs[1] = static_cast<const T*>(a.dy);
+  if constexpr (DRES) srcs[2] = static_cast<const T*>(a.res);
+  unsigned xoff[RB], dyoff[RB], dsoff[DRES ? RB : 1];
   if constexpr (TMA) {
     ring.init(ring_mem, ring_bars, D);
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
       xoff[r] = ring.thread_offset(0, CS == 1 ? r * RPC + group : r, lir);
       dyoff[r] = ring.thread_offset(1, CS == 1 ? r * RPC + group : r, lir);
+      if constexpr (DRES) dsoff[r] = ring.thread_offset(2, r * RPC + group, lir);
     }
     if (tid == 0) {
       for (int64_t k = 0; k < STAGES && k < nb; ++k)
@@ -559,7 +601,7 @@ __global__ void __launch_bounds__(RowBlock<TPR, MINB>::kBlock)
     for (int r = 0; r < RB; ++r) {
       const int64_t row = first_row + r * RPC;
       const bool rv = row < N;
-      st_mean[slot][r] = rv ? __ldg(a.mean_in + row) : 0.f;
+      if constexpr (!RMS) st_mean[slot][r] = rv ? __ldg(a.mean_in + row) : 0.f;
       st_ivar[slot][r] = rv ? __ldg(a.ivar_in + row) : 0.f;
     }
   };
@@ -575,6 +617,8 @@ __global__ void __launch_bounds__(RowBlock<TPR, MINB>::kBlock)
       if constexpr (!HOLD) {
         ring_tile<T, EPV, VPT, RB, RPC, TPR, EXACT>(stage, xoff, row0, N, nvalid, tx);
         ring_tile<T, EPV, VPT, RB, RPC, TPR, EXACT>(stage, dyoff, row0, N, nvalid, tdy);
+        if constexpr (DRES)
+          ring_tile<T, EPV, VPT, RB, RPC, TPR, EXACT>(stage, dsoff, row0, N, nvalid, tds);
       }
       if (__syncthreads_or(!ok) && !ring.dead)
         ring_give_up<decltype(ring), STAGES>(ring, a.status, j, nb,
@@ -593,6 +637,10 @@ __global__ void __launch_bounds__(RowBlock<TPR, MINB>::kBlock)
       load_tile<T, EPV, VPT, RB, RPC, VSTRIDE, EXACT>(xp, row0, N, rowvecs, nvalid, tx);
       load_tile<T, EPV, VPT, RB, RPC, VSTRIDE, EXACT>(dyp, row0, N, rowvecs, nvalid, tdy);
     }
+    // x and dy of this batch were prefetched; the third tensor is only needed after the
+    // reduction, so its loads start here and land under the sums
+    if constexpr (DRES && PF < 2)
+      load_tile<T, EPV, VPT, RB, RPC, VSTRIDE, EXACT>(dsp, row0, N, rowvecs, nvalid, tds);
     // Held ring: the batch's packed values come out of the stage, in both passes.
     auto held = [&](int r, int v, P& px, P& pdy) {
       if (row0 + r * RPC < N && (EXACT || v < nvalid)) {
@@ -608,12 +656,12 @@ __global__ void __launch_bounds__(RowBlock<TPR, MINB>::kBlock)
     // xh = (x - mean) * ivar ; gy = dy * gamma (LayerNorm) or dy (row-affine, where
     // gamma is a per-row scalar applied at the end).  red = (sum gy, sum gy * xh).
     E xh[HOLD ? 1 : RB][HOLD ? 1 : VPT][NE], gy[HOLD ? 1 : RB][HOLD ? 1 : VPT][NE];
-    float red[2 * RB];
-    float mean_of[HOLD ? RB : 1];
+    float red[NR * RB];
+    float mean_of[HOLD && !RMS ? RB : 1];
     if constexpr (!HOLD) {
 #pragma unroll
       for (int r = 0; r < RB; ++r) {
-        const float mean = st_mean[0][r];
+        const float mean = RMS ? 0.f : st_mean[0][r];
         ivar[r] = st_ivar[0][r];
         const E nm = M::bcast(-mean), iv2 = M::bcast(ivar[r]);
         E r0 = M::bcast(0.f), r1 = M::bcast(0.f);
@@ -627,28 +675,29 @@ __global__ void __launch_bounds__(RowBlock<TPR, MINB>::kBlock)
               load_param_lanes<EPV>(a.gamma, static_cast<int64_t>(vec0 + v * VSTRIDE) * EPV, gg);
 #pragma unroll
             for (int e = 0; e < NE; ++e) {
-              xh[r][v][e] = M::mul(M::add(xh[r][v][e], nm), iv2);
+              xh[r][v][e] = M::mul(RMS ? xh[r][v][e] : M::add(xh[r][v][e], nm), iv2);
               if constexpr (!ROW_AFFINE) {
                 dg[v][e] = M::fma(gy[r][v][e], xh[r][v][e], dg[v][e]);
-                db[v][e] = M::add(db[v][e], gy[r][v][e]);
+                if constexpr (!RMS) db[v][e] = M::add(db[v][e], gy[r][v][e]);
                 if constexpr (PARAMS_IN_REGS) {
                   gy[r][v][e] = M::mul(gy[r][v][e], g[v][e]);
                 } else {
                   gy[r][v][e] = M::mul(gy[r][v][e], gg[e]);
                 }
               }
-              r0 = M::add(r0, gy[r][v][e]);
+              if constexpr (!RMS) r0 = M::add(r0, gy[r][v][e]);
               r1 = M::fma(gy[r][v][e], xh[r][v][e], r1);
             }
           }
         }
-        red[2 * r] = M::hsum(r0);
-        red[2 * r + 1] = M::hsum(r1);
+        if constexpr (!RMS) red[NR * r] = M::hsum(r0);
+        red[NR * r + NR - 1] = M::hsum(r1);
       }
     } else {
 #pragma unroll
       for (int r = 0; r < RB; ++r) {
-        const float mean = mean_of[r] = st_mean[0][r];
+        const float mean = RMS ? 0.f : st_mean[0][r];
+        if constexpr (!RMS) mean_of[r] = mean;
         ivar[r] = st_ivar[0][r];
         const E nm = M::bcast(-mean), iv2 = M::bcast(ivar[r]);
         E r0 = M::bcast(0.f), r1 = M::bcast(0.f);
@@ -665,37 +714,39 @@ __global__ void __launch_bounds__(RowBlock<TPR, MINB>::kBlock)
               load_param_lanes<EPV>(a.gamma, static_cast<int64_t>(vec0 + v * VSTRIDE) * EPV, gg);
 #pragma unroll
             for (int e = 0; e < NE; ++e) {
-              xv[e] = M::mul(M::add(xv[e], nm), iv2);
+              xv[e] = M::mul(RMS ? xv[e] : M::add(xv[e], nm), iv2);
               if constexpr (!ROW_AFFINE) {
                 dg[v][e] = M::fma(gv[e], xv[e], dg[v][e]);
-                db[v][e] = M::add(db[v][e], gv[e]);
+                if constexpr (!RMS) db[v][e] = M::add(db[v][e], gv[e]);
                 if constexpr (PARAMS_IN_REGS) {
                   gv[e] = M::mul(gv[e], g[v][e]);
                 } else {
                   gv[e] = M::mul(gv[e], gg[e]);
                 }
               }
-              r0 = M::add(r0, gv[e]);
+              if constexpr (!RMS) r0 = M::add(r0, gv[e]);
               r1 = M::fma(gv[e], xv[e], r1);
             }
           }
         }
-        red[2 * r] = M::hsum(r0);
-        red[2 * r + 1] = M::hsum(r1);
+        if constexpr (!RMS) red[NR * r] = M::hsum(r0);
+        red[NR * r + NR - 1] = M::hsum(r1);
       }
     }
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
-      st_mean[0][r] = st_mean[1][r];
+      if constexpr (!RMS) {
+        st_mean[0][r] = st_mean[1][r];
+        st_mean[1][r] = st_mean[2][r];
+      }
       st_ivar[0][r] = st_ivar[1][r];
-      st_mean[1][r] = st_mean[2][r];
       st_ivar[1][r] = st_ivar[2][r];
     }
     if constexpr (PF == 1) {
       load_tile<T, EPV, VPT, RB, RPC, VSTRIDE, EXACT>(xp, row0 + stride, N, rowvecs, nvalid, tx);
       load_tile<T, EPV, VPT, RB, RPC, VSTRIDE, EXACT>(dyp, row0 + stride, N, rowvecs, nvalid, tdy);
     }
-    group_allreduce<2 * RB, TPR, BLOCK, CS>(red, sm, phase, warp, lane);
+    group_allreduce<NR * RB, TPR, BLOCK, CS>(red, sm, phase, warp, lane);
 
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
@@ -716,13 +767,22 @@ __global__ void __launch_bounds__(RowBlock<TPR, MINB>::kBlock)
         // subtraction happens before the scaling so that rows whose terms cancel
         // exactly (D == 1, constant rows) give exactly zero.
         const E sc2 = M::bcast(scale);
-        const E nm0 = M::bcast(-(red[2 * r] * inv_D));
-        const E nm1 = M::bcast(-(red[2 * r + 1] * inv_D));
+        const E nm0 = M::bcast(RMS ? 0.f : -(red[NR * r] * inv_D));
+        const E nm1 = M::bcast(-(red[NR * r + NR - 1] * inv_D));
         P* rp = dxp + row * rowvecs;
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
           if (EXACT || v < nvalid) {
-            E o[NE];
+            E o[NE], ds[NE];
+            if constexpr (DRES) {
+              P pds;
+              if constexpr (HOLD) {
+                pds = reinterpret_cast<const P*>(stage + dsoff[r])[v * TPR];
+              } else {
+                pds = tds.p[r][v];
+              }
+              unpack<T, EPV>(pds, ds);
+            }
             if constexpr (HOLD) {
               // second pass over the batch, again out of the ring stage
               E xv[NE], gv[NE], gg[NE];
@@ -732,10 +792,10 @@ __global__ void __launch_bounds__(RowBlock<TPR, MINB>::kBlock)
               unpack<T, EPV>(pdy, gv);
               if constexpr (!ROW_AFFINE && !PARAMS_IN_REGS)
                 load_param_lanes<EPV>(a.gamma, static_cast<int64_t>(vec0 + v * VSTRIDE) * EPV, gg);
-              const E nm = M::bcast(-mean_of[r]), iv2 = M::bcast(ivar[r]);
+              const E nm = M::bcast(RMS ? 0.f : -mean_of[RMS ? 0 : r]), iv2 = M::bcast(ivar[r]);
 #pragma unroll
               for (int e = 0; e < NE; ++e) {
-                xv[e] = M::mul(M::add(xv[e], nm), iv2);
+                xv[e] = M::mul(RMS ? xv[e] : M::add(xv[e], nm), iv2);
                 if constexpr (!ROW_AFFINE) {
                   if constexpr (PARAMS_IN_REGS) {
                     gv[e] = M::mul(gv[e], g[v][e]);
@@ -743,12 +803,23 @@ __global__ void __launch_bounds__(RowBlock<TPR, MINB>::kBlock)
                     gv[e] = M::mul(gv[e], gg[e]);
                   }
                 }
-                o[e] = M::mul(M::add(gv[e], M::fma(xv[e], nm1, nm0)), sc2);
+                if constexpr (RMS) {
+                  o[e] = M::fma(xv[e], nm1, gv[e]);
+                } else {
+                  o[e] = M::add(gv[e], M::fma(xv[e], nm1, nm0));
+                }
+                o[e] = DRES ? M::fma(o[e], sc2, ds[e]) : M::mul(o[e], sc2);
               }
             } else {
 #pragma unroll
-              for (int e = 0; e < NE; ++e)
-                o[e] = M::mul(M::add(gy[r][v][e], M::fma(xh[r][v][e], nm1, nm0)), sc2);
+              for (int e = 0; e < NE; ++e) {
+                if constexpr (RMS) {
+                  o[e] = M::fma(xh[r][v][e], nm1, gy[r][v][e]);
+                } else {
+                  o[e] = M::add(gy[r][v][e], M::fma(xh[r][v][e], nm1, nm0));
+                }
+                o[e] = DRES ? M::fma(o[e], sc2, ds[e]) : M::mul(o[e], sc2);
+              }
             }
             store_stream<T, EPV>(reinterpret_cast<T*>(rp + v * VSTRIDE), 0, repack<T, EPV>(o));
           }
@@ -758,8 +829,8 @@ __global__ void __launch_bounds__(RowBlock<TPR, MINB>::kBlock)
   }
 
   if constexpr (!ROW_AFFINE) {
-    float* __restrict__ wg = a.ws + (unit * 2 + 0) * D;
-    float* __restrict__ wb = a.ws + (unit * 2 + 1) * D;
+    float* __restrict__ wg = a.ws + unit * NR * D;
+    float* __restrict__ wb = wg + D;  // not used by RMS
     if constexpr (RPC > 1) {
       // Fold the row groups of this CTA in group order, then group 0 writes.
       float* cg_ = comb;
@@ -774,15 +845,17 @@ __global__ void __launch_bounds__(RowBlock<TPR, MINB>::kBlock)
               if constexpr (EPV == 1) {
                 const int idx = v * TPR + lir;
                 cg_[idx] = (rgrp == 0 ? 0.f : cg_[idx]) + dg[v][e];
-                cb_[idx] = (rgrp == 0 ? 0.f : cb_[idx]) + db[v][e];
+                if constexpr (!RMS) cb_[idx] = (rgrp == 0 ? 0.f : cb_[idx]) + db[v][e];
               } else {
                 float2* cg2 = reinterpret_cast<float2*>(cg_);
                 float2* cb2 = reinterpret_cast<float2*>(cb_);
                 const int idx = (v * NE + e) * TPR + lir;
                 float2 pg = rgrp == 0 ? make_float2(0.f, 0.f) : cg2[idx];
-                float2 pb = rgrp == 0 ? make_float2(0.f, 0.f) : cb2[idx];
                 cg2[idx] = make_float2(pg.x + dg[v][e].x, pg.y + dg[v][e].y);
-                cb2[idx] = make_float2(pb.x + db[v][e].x, pb.y + db[v][e].y);
+                if constexpr (!RMS) {
+                  float2 pb = rgrp == 0 ? make_float2(0.f, 0.f) : cb2[idx];
+                  cb2[idx] = make_float2(pb.x + db[v][e].x, pb.y + db[v][e].y);
+                }
               }
             }
         }
@@ -795,10 +868,10 @@ __global__ void __launch_bounds__(RowBlock<TPR, MINB>::kBlock)
           for (int e = 0; e < NE; ++e) {
             if constexpr (EPV == 1) {
               dg[v][e] = cg_[v * TPR + lir];
-              db[v][e] = cb_[v * TPR + lir];
+              if constexpr (!RMS) db[v][e] = cb_[v * TPR + lir];
             } else {
               dg[v][e] = reinterpret_cast<float2*>(cg_)[(v * NE + e) * TPR + lir];
-              db[v][e] = reinterpret_cast<float2*>(cb_)[(v * NE + e) * TPR + lir];
+              if constexpr (!RMS) db[v][e] = reinterpret_cast<float2*>(cb_)[(v * NE + e) * TPR + lir];
             }
           }
       }
@@ -808,7 +881,8 @@ __global__ void __launch_bounds__(RowBlock<TPR, MINB>::kBlock)
       for (int v = 0; v < VPT; ++v) {
         if (EXACT || v < nvalid) {
           store_param_lanes<EPV>(wg, static_cast<int64_t>(vec0 + v * VSTRIDE) * EPV, dg[v]);
-          store_param_lanes<EPV>(wb, static_cast<int64_t>(vec0 + v * VSTRIDE) * EPV, db[v]);
+          if constexpr (!RMS)
+            store_param_lanes<EPV>(wb, static_cast<int64_t>(vec0 + v * VSTRIDE) * EPV, db[v]);
         }
       }
     }

@@ -161,6 +161,43 @@ NVN_API int nvn_ln_bwd(int dtype, const void* dy, const void* x, const float* ga
                        void* dx, float* dgamma, float* dbeta, void* workspace,
                        size_t workspace_bytes, void* stream);
 
+/* LayerNorm gradient with the gradient of the residual stream: as nvn_ln_bwd, where x is the
+ * sum that nvn_ln_fwd_residual wrote and dsum [N, D] of T is the gradient that reaches that
+ * sum from the residual branch,
+ *   dx_ij = T(nvn_ln_bwd's dx_ij in fp32 + dsum_ij)     (one rounding)
+ * dx may alias dsum (the stream's gradient updated in place).  Rows of any width.
+ * No counterpart in the reference. */
+NVN_API size_t nvn_ln_bwd_residual_workspace_bytes(int dtype, int64_t N, int64_t D);
+NVN_API int nvn_ln_bwd_residual(int dtype, const void* dy, const void* dsum, const void* x,
+                                const float* gamma, const float* mean, const float* inv_std,
+                                int64_t N, int64_t D, void* dx, float* dgamma, float* dbeta,
+                                void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- RMS normalisation --------------------------------------------------------
+ * x, y: [N, D] of T, row-major.  gamma: [D] fp32.  inv_rms: [N] fp32 or NULL (not saved).
+ *   inv_rms_i = 1 / sqrt(sum_j x_ij^2 / D + epsilon)
+ *   y_ij      = x_ij inv_rms_i gamma_j
+ * y may alias x.  No workspace.  The residual form normalises s_ij = T(x_ij + residual_ij),
+ * which it also writes; sum_out may alias x or residual, y may alias x or residual, and
+ * sum_out and y must not overlap.  Rows of any width.  No counterpart in the reference. */
+NVN_API int nvn_rms_fwd(int dtype, const void* x, const float* gamma, int64_t N, int64_t D,
+                        float epsilon, void* y, float* inv_rms, void* stream);
+NVN_API int nvn_rms_fwd_residual(int dtype, const void* x, const void* residual,
+                                 const float* gamma, int64_t N, int64_t D, float epsilon,
+                                 void* sum_out, void* y, float* inv_rms, void* stream);
+
+/* dy, x, dx: [N, D] of T.  dgamma: [D] fp32.  dsum: [N, D] of T, the gradient that reaches x
+ * from a residual branch, or NULL.
+ *   xh_ij    = x_ij inv_rms_i
+ *   dgamma_j = sum_i dy_ij xh_ij                       (fixed order: the same bits every run)
+ *   dx_ij    = T(inv_rms_i (dy_ij gamma_j - xh_ij sum_k(dy_ik gamma_k xh_ik) / D) + dsum_ij)
+ * dx may alias dsum. */
+NVN_API size_t nvn_rms_bwd_workspace_bytes(int dtype, int64_t N, int64_t D);
+NVN_API int nvn_rms_bwd(int dtype, const void* dy, const void* dsum, const void* x,
+                        const float* gamma, const float* inv_rms, int64_t N, int64_t D,
+                        void* dx, float* dgamma, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
 /* ---- InstanceNorm -----------------------------------------------------------
  * x, y: [N, C, D] (channel_first != 0, "NC...") or [N, D, C] ("N...C") of T.
  * gamma, beta: [C] fp32.  mean, inv_std: [N, C] fp32.  Statistics are taken
