@@ -13,6 +13,8 @@ LIB_PATH = os.path.join(_HERE, "libnvnorms.so")
 
 NVN_F32, NVN_F16, NVN_BF16 = 0, 1, 2
 
+NVN_NORM_NONE, NVN_NORM_RMS, NVN_NORM_LAYER = 0, 1, 2
+
 NVN_OK = 0
 NVN_ERR_INVALID_ARGUMENT = -1
 NVN_ERR_AXIS_RANGE = -2
@@ -77,6 +79,9 @@ SIGNATURES = {
     "nvn_rms_fwd_residual": (_int, [_int, _vp, _vp, _vp, _i64, _i64, _c.c_float, _vp, _vp, _vp, _vp]),
     "nvn_rms_bwd_workspace_bytes": (_sz, [_int, _i64, _i64]),
     "nvn_rms_bwd": (_int, [_int, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _sz, _vp]),
+    "nvn_head_norm_rotary_fwd": (_int, [_vp, _vp, _vp, _vp]),
+    "nvn_head_norm_rotary_bwd_workspace_bytes": (_sz, [_vp]),
+    "nvn_head_norm_rotary_bwd": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "nvn_ln_bwd_noalloc": (_int, [_int, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp]),
     "nvn_in_bwd_dp": (_int, [_int, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _vp, _vp, _vp,
                              _vp, _sz, _c.POINTER(DpComm), _vp]),

@@ -39,6 +39,7 @@ def _units():
             units.append((f"rows_{tname}_{dname}.o", "rows_inst.cu", [f"-DNVN_T={t}", f"-DNVN_BWD={b}"]))
             units.append((f"rows_rms_{tname}_{dname}.o", "rows_rms_inst.cu",
                           [f"-DNVN_T={t}", f"-DNVN_BWD={b}"]))
+            units.append((f"heads_{tname}_{dname}.o", "heads_inst.cu", [f"-DNVN_T={t}", f"-DNVN_BWD={b}"]))
         units.append((f"rows_res_{tname}.o", "rows_res_inst.cu", [f"-DNVN_T={t}"]))
     units.append(("rows_wide.o", "rows_wide.cu", []))
     units.append(("twophase.o", "twophase.cu", []))
@@ -50,6 +51,7 @@ def _units():
     units.append(("nvnorms_api.o", "nvnorms_api.cu", []))
     units.append(("rows_generic.o", "rows_generic.cu", []))
     units.append(("rms_api.o", "rms_api.cu", []))
+    units.append(("heads_api.o", "heads_api.cu", []))
     units.append(("noalloc.o", "noalloc.cu", []))
     return units
 

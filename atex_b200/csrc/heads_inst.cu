@@ -1,0 +1,122 @@
+// Instantiates the per-head normalisation and rotary kernels (head_rotary.cuh) for one
+// (dtype, direction) pair; compiled six times with -DNVN_T={0,1,2} and -DNVN_BWD={0,1}.
+#include "head_rotary.cuh"
+
+#if NVN_T == 0
+using T = float;
+#define NVN_TNAME f32
+#elif NVN_T == 1
+using T = __half;
+#define NVN_TNAME f16
+#else
+using T = __nv_bfloat16;
+#define NVN_TNAME bf16
+#endif
+
+#if NVN_BWD
+#define NVN_DIR bwd
+#else
+#define NVN_DIR fwd
+#endif
+
+#define NVN_CAT3_(a, b, c) a##_##b##_##c
+#define NVN_CAT3(a, b, c) NVN_CAT3_(a, b, c)
+
+namespace nvn {
+
+namespace {
+
+constexpr bool kBwd = NVN_BWD != 0;
+constexpr int kTableBytes = 32 * 1024;   // most a tile's cosines and sines may take
+
+inline int round4(int v) { return (v + 3) / 4 * 4; }
+
+template <int V, int NORM, bool IL>
+cudaError_t launch(HeadArgs& a, cudaStream_t s, bool dry_run, HeadPlan* plan) {
+  auto kernel = head_kernel<T, V, NORM, IL, kBwd>;
+  constexpr int SPT = HeadTraits<T, V>::SPT;
+  constexpr int NV = NORM == 0 ? 0 : (NORM == 1 ? 1 : 2);
+  constexpr int R = (kBwd ? 2 : 4) / (sizeof(T) == 4 ? 2 : 1);
+  const int slots = (a.hd + 2 * V - 1) / (2 * V);
+  a.tph = 1;
+  while (a.tph * SPT < slots) a.tph *= 2;
+  if (a.tph > 32) return cudaErrorInvalidValue;
+  a.pstride = round4(a.pairs > 0 ? a.pairs : 1);
+  a.hd4 = round4(a.hd);
+  // A tile holds two batches of rows for every group, less when that leaves SMs without a CTA.
+  const int heads = a.part[0].heads + (a.parts > 1 ? a.part[1].heads : 0);
+  const int groups = kHeadBlock / a.tph;
+  int64_t tile = heads > 0 ? (2 * R * groups + heads - 1) / heads : 1;
+  const int64_t spread = a.N / (static_cast<int64_t>(device_sm_count()) * 4);
+  if (tile > spread) tile = spread;
+  const int64_t most = kTableBytes / (8 * a.pstride);
+  if (tile > most) tile = most;
+  a.tile = static_cast<int>(tile < 1 ? 1 : tile);
+  a.tiles = (a.N + a.tile - 1) / a.tile;
+  const size_t smem = (static_cast<size_t>(2) * a.tile * a.pstride + 2 * NV * a.hd4 +
+                       (kBwd ? 2 * NV * 16 * kHeadBlock : 0)) * 4;
+  static std::atomic<uint64_t> prepared{0};
+  cudaError_t e = once_per_device(prepared, [&]() -> cudaError_t {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                kTableBytes + (2 * NV * 512 + (kBwd ? 2 * NV * 16 * kHeadBlock : 0)) * 4);
+  });
+  if (e != cudaSuccess) return e;
+  int64_t grid = a.tiles;
+  if (kBwd) {   // persistent: the parameter sums stay in the CTA over all its tiles
+    static std::atomic<int64_t> cached{0};  // (shared bytes << 20) | CTAs per SM
+    const int64_t c = cached.load(std::memory_order_relaxed);
+    int per_sm = 0;
+    if (c != 0 && static_cast<size_t>(c >> 20) == smem) {
+      per_sm = static_cast<int>(c & 0xfffff);
+    } else {
+      e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kHeadBlock, smem);
+      if (e != cudaSuccess) return e;
+      if (per_sm < 1) per_sm = 1;
+      cached.store((static_cast<int64_t>(smem) << 20) | per_sm, std::memory_order_relaxed);
+    }
+    const int64_t resident = static_cast<int64_t>(per_sm) * device_sm_count();
+    if (grid > resident) grid = resident;
+  }
+  plan->v = V;
+  plan->grid = static_cast<int>(grid);
+  plan->smem = smem;
+  if (dry_run) return cudaSuccess;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
+  cfg.blockDim = dim3(kHeadBlock, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  // dependent launches for short kernels only, as for the row kernels
+  attr[0].val.programmaticStreamSerializationAllowed =
+      use_dependent_launch() &&
+              a.N * heads * a.hd * static_cast<int64_t>(sizeof(T)) <= (int64_t(128) << 20)
+          ? 1
+          : 0;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  count_launch();
+  return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
+template <int V>
+cudaError_t launch_v(int norm, bool il, HeadArgs& a, cudaStream_t s, bool dry, HeadPlan* plan) {
+  if (norm == 0) return il ? launch<V, 0, true>(a, s, dry, plan) : launch<V, 0, false>(a, s, dry, plan);
+  if (norm == 1) return il ? launch<V, 1, true>(a, s, dry, plan) : launch<V, 1, false>(a, s, dry, plan);
+  return il ? launch<V, 2, true>(a, s, dry, plan) : launch<V, 2, false>(a, s, dry, plan);
+}
+
+}  // namespace
+
+cudaError_t NVN_CAT3(heads, NVN_TNAME, NVN_DIR)(int norm, bool interleaved, int v, HeadArgs& a,
+                                                 cudaStream_t s, bool dry_run, HeadPlan* plan) {
+  if constexpr (VecTraits<T>::kFull == 8) {
+    if (v == 8) return launch_v<8>(norm, interleaved, a, s, dry_run, plan);
+  }
+  if (v == 4) return launch_v<4>(norm, interleaved, a, s, dry_run, plan);
+  if (v == 2) return launch_v<2>(norm, interleaved, a, s, dry_run, plan);
+  return launch_v<1>(norm, interleaved, a, s, dry_run, plan);
+}
+
+}  // namespace nvn

@@ -303,18 +303,57 @@ int generic_slices(int64_t N, int64_t D, int epv);
 cudaError_t generic_launch(int dtype, bool vec, bool bwd, bool rms, const RowsResArgs& a,
                            float* coef, int slices, cudaStream_t s);
 
-// out[c] = sum over `rows` partial rows of `cols` floats, in a fixed order; one or two
-// segments of the same width in one launch (launched as a dependent of the kernel before it).
-struct ColsumSegment {
-  const float* partials;
-  float* out;
-  int64_t rows;
+// out[c] = sum over `rows` partial rows of `cols` floats, in a fixed order (launched as a
+// dependent of the kernel before it).
+cudaError_t colsum_launch(const float* partials, int64_t rows, int64_t cols, float* out,
+                          cudaStream_t s);
+
+// Per-head normalisation with rotary positions (head_rotary.cuh).  Strides are in elements,
+// in the order batch, token, head; the elements of a head are contiguous.
+struct HeadDiv {   // division by a fixed number: see fast_div
+  unsigned mul;
+  int shift;       // < 0: the divisor is 1
 };
-struct ColsumArgs {
-  ColsumSegment seg[2];
-  int64_t cols;
+struct HeadPart {  // the queries or the keys
+  const void* x;
+  const void* dy;
+  void* out;
+  int64_t xs[3], ds[3], os[3];
+  int heads;
+  HeadDiv div;     // by heads
 };
-cudaError_t colsum_launch(const ColsumArgs& a, int segments, cudaStream_t s);
+struct HeadArgs {
+  HeadPart part[2];
+  int parts;
+  const float* param[4];  // scale and offset of the queries, scale and offset of the keys
+  float* ws;              // partial rows [grid][parts][1 or 2][hd]
+  const void* positions;
+  const double* inv_freq;
+  const int32_t* pair_axis;
+  int64_t ps[3];          // strides of positions: axis, batch, token
+  int pos64, axes, pairs;
+  int64_t N, T, tiles;    // N = batch * tokens
+  HeadDiv tdiv;           // by T
+  int hd, hd4, tph, tile, pstride;
+  float inv_hd, eps;
+};
+struct HeadPlan {
+  int v;                  // elements per access
+  int grid;               // CTAs = partial rows
+  size_t smem;
+};
+// `bwd`, `norm` (0 none, 1 root mean square, 2 mean and variance), `interleaved` select the
+// kernel; a.part / a.tile ... are filled in by the caller except tile, tiles, pstride, hd4, tph,
+// which the plan sets.  With dry_run nothing is launched.
+#define NVN_DECLARE_HEADS(NAME)                                                                \
+  cudaError_t NAME(int norm, bool interleaved, int v, HeadArgs& a, cudaStream_t s, bool dry_run, \
+                   HeadPlan* plan);
+NVN_DECLARE_HEADS(heads_f32_fwd)
+NVN_DECLARE_HEADS(heads_f32_bwd)
+NVN_DECLARE_HEADS(heads_f16_fwd)
+NVN_DECLARE_HEADS(heads_f16_bwd)
+NVN_DECLARE_HEADS(heads_bf16_fwd)
+NVN_DECLARE_HEADS(heads_bf16_bwd)
 
 // Deterministic second stage of the dgamma / dbeta reduction: sums P partial
 // rows of [2][F] floats (dgamma then dbeta) in a fixed order.

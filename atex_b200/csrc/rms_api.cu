@@ -154,10 +154,7 @@ int backward(int form, int dtype, const void* dy, const void* dsum, const void* 
   if (form == 2) {
     e = colreduce_launch(a.ws, p.partial_rows, D, dgamma, dbeta, s);
   } else {
-    ColsumArgs c = {};
-    c.seg[0] = {a.ws, dgamma, p.partial_rows};
-    c.cols = D;
-    e = colsum_launch(c, 1, s);
+    e = colsum_launch(a.ws, p.partial_rows, D, dgamma, s);
   }
   return e == cudaSuccess ? NVN_OK : fail_cuda(e);
 }

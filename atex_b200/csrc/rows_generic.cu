@@ -229,35 +229,35 @@ cudaError_t generic_t(bool vec, bool bwd, bool rms, const RowsResArgs& a, float*
 constexpr int kSumX = 32;
 
 template <int TY>
-__global__ void __launch_bounds__(kSumX* TY) colsum_kernel(const ColsumArgs a) {
+__global__ void __launch_bounds__(kSumX* TY)
+    colsum_kernel(const float* __restrict__ partials, int64_t rows, int64_t cols,
+                  float* __restrict__ out) {
   __shared__ float tile[TY][kSumX + 1];
   const int tx = threadIdx.x, ty = threadIdx.y;
-  const ColsumSegment seg = blockIdx.y == 0 ? a.seg[0] : a.seg[1];
   const int64_t col = static_cast<int64_t>(blockIdx.x) * kSumX + tx;
   griddep_launch_dependents();
   griddep_wait();  // the partial rows come from the kernel launched just before
   float s = 0.f;
-  if (col < a.cols) {
-    for (int64_t p = ty; p < seg.rows; p += TY) s += seg.partials[p * a.cols + col];
+  if (col < cols) {
+    for (int64_t p = ty; p < rows; p += TY) s += partials[p * cols + col];
   }
   tile[ty][tx] = s;
   __syncthreads();
-  if (ty == 0 && col < a.cols) {
+  if (ty == 0 && col < cols) {
     float t = 0.f;
 #pragma unroll
     for (int k = 0; k < TY; ++k) t += tile[k][tx];
-    seg.out[col] = t;
+    out[col] = t;
   }
 }
 
 template <int TY>
-cudaError_t colsum_t(const ColsumArgs& a, int segments, cudaStream_t s) {
+cudaError_t colsum_t(const float* partials, int64_t rows, int64_t cols, float* out, cudaStream_t s) {
   cudaLaunchAttribute attr;
   const cudaLaunchConfig_t cfg = dependent_launch_config(
-      dim3(static_cast<unsigned>((a.cols + kSumX - 1) / kSumX), static_cast<unsigned>(segments)),
-      dim3(kSumX, TY), 0, s, &attr);
+      dim3(static_cast<unsigned>((cols + kSumX - 1) / kSumX)), dim3(kSumX, TY), 0, s, &attr);
   count_launch();
-  return cudaLaunchKernelEx(&cfg, colsum_kernel<TY>, a);
+  return cudaLaunchKernelEx(&cfg, colsum_kernel<TY>, partials, rows, cols, out);
 }
 
 }  // namespace
@@ -277,9 +277,10 @@ cudaError_t generic_launch(int dtype, bool vec, bool bwd, bool rms, const RowsRe
   return generic_t<__nv_bfloat16>(vec, bwd, rms, a, coef, slices, s);
 }
 
-cudaError_t colsum_launch(const ColsumArgs& a, int segments, cudaStream_t s) {
-  const int64_t rows = segments > 1 && a.seg[1].rows > a.seg[0].rows ? a.seg[1].rows : a.seg[0].rows;
-  return rows <= 32 ? colsum_t<4>(a, segments, s) : colsum_t<32>(a, segments, s);
+cudaError_t colsum_launch(const float* partials, int64_t rows, int64_t cols, float* out,
+                          cudaStream_t s) {
+  return rows <= 32 ? colsum_t<4>(partials, rows, cols, out, s)
+                    : colsum_t<32>(partials, rows, cols, out, s);
 }
 
 }  // namespace nvn

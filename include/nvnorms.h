@@ -198,6 +198,71 @@ NVN_API int nvn_rms_bwd(int dtype, const void* dy, const void* dsum, const void*
                         void* dx, float* dgamma, void* workspace, size_t workspace_bytes,
                         void* stream);
 
+/* ---- per-head normalisation and rotary positions -------------------------------
+ * Attention queries and keys [batch, token, head, head_dim] of T, read once, normalised over
+ * head_dim, rotated and written once.  With c = x (RMS) or x - mean(x) (LAYER):
+ *   n = c / sqrt(mean(c^2) + epsilon) scale (+ offset for LAYER);   NONE: n = x
+ *   pair p turns by angle = position[pair_axis[p], batch, token] inv_freq[p]:
+ *   (u, v) -> (u cos - v sin, u sin + v cos)
+ * Pair p is the elements (p, p + pairs) of a head, or (2p, 2p + 1) when `interleaved`; elements
+ * from 2 pairs on are normalised and not rotated.  Angles are formed in 64 bits, everything
+ * else in fp32, with one rounding to T.  A pair whose axis is not in [0, axes) is not rotated.
+ *   - nvn_heads: a view.  The elements of a head are contiguous, the three strides (in
+ *     elements) are free: a slice of a packed projection, head-major tensors and so on.  An
+ *     output may be the input's own view (in place); otherwise outputs overlap nothing.
+ *   - k.data NULL: queries alone.  pairs 0: no rotation (positions, inv_freq, pair_axis unused).
+ *   - head_dim <= 512 (NVN_ERR_LIMIT beyond), at most 65535 heads, batch * tokens < 2^31.
+ *   - positions: int32 or int64 (position_bytes 4 or 8), [axes, batch, token] with free strides
+ *     (0 to share); inv_freq: [pairs] radians per position; pair_axis: [pairs].
+ * No counterpart in the reference. */
+typedef enum nvn_head_norm { NVN_NORM_NONE = 0, NVN_NORM_RMS = 1, NVN_NORM_LAYER = 2 } nvn_head_norm;
+
+typedef struct nvn_heads {
+  void* data;
+  int64_t heads;
+  int64_t stride_batch;
+  int64_t stride_token;
+  int64_t stride_head;
+} nvn_heads;
+
+typedef struct nvn_head_problem {
+  int32_t dtype;
+  int32_t norm;        /* nvn_head_norm */
+  int32_t interleaved;
+  float epsilon;
+  int64_t batch;
+  int64_t tokens;
+  int64_t head_dim;
+  int64_t pairs;
+  int32_t axes;
+  int32_t position_bytes;
+  const void* positions;
+  int64_t position_stride_axis;
+  int64_t position_stride_batch;
+  int64_t position_stride_token;
+  const double* inv_freq;
+  const int32_t* pair_axis;
+  nvn_heads q;
+  nvn_heads k;
+  const float* scale_q;  /* [head_dim] fp32 */
+  const float* offset_q;
+  const float* scale_k;
+  const float* offset_k;
+} nvn_head_problem;
+
+NVN_API int nvn_head_norm_rotary_fwd(const nvn_head_problem* problem, const nvn_heads* q_out,
+                                     const nvn_heads* k_out, void* stream);
+
+/* Gradient: q_grad / k_grad reach the outputs, dq / dk are written (views of q's and k's shape;
+ * dq may be q_grad's own view).  The statistics are formed again from q and k.  dparams: fp32,
+ * [parts][vectors][head_dim] with parts = q (and k), vectors = scale (and offset for LAYER);
+ * unused for NONE.  The sums over batch, tokens and heads have a fixed order. */
+NVN_API size_t nvn_head_norm_rotary_bwd_workspace_bytes(const nvn_head_problem* problem);
+NVN_API int nvn_head_norm_rotary_bwd(const nvn_head_problem* problem, const nvn_heads* q_grad,
+                                     const nvn_heads* k_grad, const nvn_heads* dq,
+                                     const nvn_heads* dk, float* dparams, void* workspace,
+                                     size_t workspace_bytes, void* stream);
+
 /* ---- InstanceNorm -----------------------------------------------------------
  * x, y: [N, C, D] (channel_first != 0, "NC...") or [N, D, C] ("N...C") of T.
  * gamma, beta: [C] fp32.  mean, inv_std: [N, C] fp32.  Statistics are taken
