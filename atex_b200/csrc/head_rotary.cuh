@@ -20,11 +20,15 @@
 //   behind the rotated elements a slot is 2V plain elements.
 // In every form slot s turns by the V angles from pair sV on.
 //
-// A CTA takes a tile of consecutive tokens with all their heads, queries and keys: the angles of
-// a token are the same for all of them and are computed once per tile into shared memory - in 64
+// A CTA takes tiles of consecutive tokens with all their heads, queries and keys: the angles of a
+// token are the same for all of them and are computed once per tile into shared memory - in 64
 // bits up to the fraction of a turn, because a position of a million times a frequency has no
-// fraction left in 32.  The rows of the tile are dealt to the groups of TPH lanes; each group
-// keeps R rows in flight, and those of the first batch are fetched before the angles are computed.
+// fraction left in 32.  The rows of a tile are dealt to the groups of TPH lanes; while a group
+// works on a row its next one is already on the way into registers, across the ends of parts and
+// tiles too.  The tables (angles, and the element offsets of the tokens) have three buffers, so
+// that one barrier per tile is enough: tile i reads buffer i, its last rows fetch from the offsets
+// of buffer i + 1, and the barrier in tile i + 1 stands between the last read of buffer i and its
+// refill in tile i + 2.
 #pragma once
 
 #include "nvn_common.cuh"
@@ -40,10 +44,11 @@ __device__ __forceinline__ unsigned fast_div(unsigned n, const HeadDiv& d) {
   return d.shift < 0 ? n : __umulhi(n, d.mul) >> d.shift;
 }
 
-template <typename T, int V>
+template <int V>
 struct HeadTraits {
-  static constexpr int SPT = 8 / V;                       // slots per thread
-  using P = Pack<T, V>;
+  static constexpr int SPT = 8 / V;             // slots per thread
+  static constexpr int CW = V < 4 ? V : 4;      // floats of one access to the angle table
+  static constexpr int CHUNKS = V / CW;         // accesses for a slot's cosines
 };
 
 // Element column of vector `half` of slot s.
@@ -53,39 +58,78 @@ __device__ __forceinline__ int head_col(int s, int half, int pairs) {
   return (2 * s + half) * V;
 }
 
-// (a, b) -> (a cos - b sin, a sin + b cos), or the other way round for SIGN < 0; `c`, `sn` are the
-// V cosines and sines of the slot.
-template <int V, bool IL, int SIGN>
-__device__ __forceinline__ void head_turn(float (&a)[V], float (&b)[V], const float* c,
-                                          const float* sn, bool rot_a, bool rot_b) {
+// Angle table of one token: [cos, sin][chunk][slot][CW], so that neighbouring lanes read
+// neighbouring 16-byte words.
+template <int V>
+__device__ __forceinline__ int head_table_at(int p, bool sine, int nslots) {
+  constexpr int CW = HeadTraits<V>::CW, CHUNKS = HeadTraits<V>::CHUNKS;
+  const int s = p / V, e = p % V;
+  return (((sine ? CHUNKS : 0) + e / CW) * nslots + s) * CW + e % CW;
+}
+
+// The V cosines (or sines) of slot s.
+template <int V>
+__device__ __forceinline__ void head_table_read(const float* tab, bool sine, int s, int nslots,
+                                                float (&out)[V]) {
+  constexpr int CW = HeadTraits<V>::CW, CHUNKS = HeadTraits<V>::CHUNKS;
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    const float* p = tab + (((sine ? CHUNKS : 0) + c) * nslots + s) * CW;
+    if constexpr (CW == 4) {
+      const float4 v = *reinterpret_cast<const float4*>(p);
+      out[4 * c] = v.x;
+      out[4 * c + 1] = v.y;
+      out[4 * c + 2] = v.z;
+      out[4 * c + 3] = v.w;
+    } else if constexpr (CW == 2) {
+      const float2 v = *reinterpret_cast<const float2*>(p);
+      out[0] = v.x;
+      out[1] = v.y;
+    } else {
+      out[0] = *p;
+    }
+  }
+}
+
+__device__ __forceinline__ float2 neg(float2 v) { return make_float2(-v.x, -v.y); }
+__device__ __forceinline__ float neg(float v) { return -v; }
+
+// (a, b) -> (a cos - b sin, a sin + b cos), turned back for SIGN < 0.
+template <int V, bool IL, int SIGN, typename E, int NE>
+__device__ __forceinline__ void head_turn(E (&a)[NE], E (&b)[NE], const float (&c)[V],
+                                          const float (&sn)[V], bool rot_a, bool rot_b) {
+  using M = typename MathSel<V>::M;
   if constexpr (!IL || V == 1) {
     if (rot_a) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float s = SIGN > 0 ? sn[e] : -sn[e];
-        const float u = fmaf(a[e], c[e], -(b[e] * s));
-        b[e] = fmaf(a[e], s, b[e] * c[e]);
-        a[e] = u;
+      for (int e = 0; e < NE; ++e) {
+        E cc, ss;
+        if constexpr (V == 1) {
+          cc = c[0];
+          ss = sn[0];
+        } else {
+          cc = make_float2(c[2 * e], c[2 * e + 1]);
+          ss = make_float2(sn[2 * e], sn[2 * e + 1]);
+        }
+        const E bs = M::mul(b[e], ss), as = M::mul(a[e], ss);
+        a[e] = M::fma(a[e], cc, SIGN > 0 ? neg(bs) : bs);
+        b[e] = M::fma(b[e], cc, SIGN > 0 ? as : neg(as));
       }
     }
   } else {
+    auto turn = [&](E& v, float cc, float ss) {
+      if (SIGN < 0) ss = -ss;
+      const float u = fmaf(v.x, cc, -(v.y * ss));
+      v.y = fmaf(v.x, ss, v.y * cc);
+      v.x = u;
+    };
     if (rot_a) {
 #pragma unroll
-      for (int e = 0; e < V; e += 2) {
-        const float s = SIGN > 0 ? sn[e / 2] : -sn[e / 2];
-        const float u = fmaf(a[e], c[e / 2], -(a[e + 1] * s));
-        a[e + 1] = fmaf(a[e], s, a[e + 1] * c[e / 2]);
-        a[e] = u;
-      }
+      for (int e = 0; e < NE; ++e) turn(a[e], c[e], sn[e]);
     }
     if (rot_b) {
 #pragma unroll
-      for (int e = 0; e < V; e += 2) {
-        const float s = SIGN > 0 ? sn[(V + e) / 2] : -sn[(V + e) / 2];
-        const float u = fmaf(b[e], c[(V + e) / 2], -(b[e + 1] * s));
-        b[e + 1] = fmaf(b[e], s, b[e + 1] * c[(V + e) / 2]);
-        b[e] = u;
-      }
+      for (int e = 0; e < NE; ++e) turn(b[e], c[NE + e], sn[NE + e]);
     }
   }
 }
@@ -101,52 +145,98 @@ __device__ __forceinline__ void head_reduce(float (&v)[N], int tph) {
   }
 }
 
-template <typename T, int V>
-__device__ __forceinline__ void head_unpack(const Pack<T, V>& p, float (&f)[V]) {
-  typename MathSel<V>::M::E lanes[MathSel<V>::NE];
-  unpack<T, V>(p, lanes);
-  if constexpr (V == 1) {
-    f[0] = lanes[0];
-  } else {
+// V consecutive floats of shared memory as math lanes.
+template <int V>
+__device__ __forceinline__ void head_lanes(const float* p, typename MathSel<V>::M::E (&out)[MathSel<V>::NE]) {
+  if constexpr (V % 4 == 0) {
 #pragma unroll
-    for (int i = 0; i < V / 2; ++i) {
-      f[2 * i] = lanes[i].x;
-      f[2 * i + 1] = lanes[i].y;
+    for (int i = 0; i < V / 4; ++i) {
+      const float4 v = reinterpret_cast<const float4*>(p)[i];
+      out[2 * i] = make_float2(v.x, v.y);
+      out[2 * i + 1] = make_float2(v.z, v.w);
+    }
+  } else if constexpr (V == 2) {
+    out[0] = *reinterpret_cast<const float2*>(p);
+  } else {
+    out[0] = *p;
+  }
+}
+
+// The same, to shared memory of a thread's own: element e of vector j is word
+// ((j V + e) / CW) CW kHeadBlock + CW thread + e % CW, so that a warp's accesses are contiguous.
+template <int V>
+__device__ __forceinline__ void head_sums_load(const float* p, int j, typename MathSel<V>::M::E (&out)[MathSel<V>::NE]) {
+  constexpr int CW = HeadTraits<V>::CW;
+#pragma unroll
+  for (int c = 0; c < V / CW; ++c) {
+    const float* q = p + (j * (V / CW) + c) * CW * kHeadBlock;
+    if constexpr (CW == 4) {
+      const float4 v = *reinterpret_cast<const float4*>(q);
+      out[2 * c] = make_float2(v.x, v.y);
+      out[2 * c + 1] = make_float2(v.z, v.w);
+    } else if constexpr (CW == 2) {
+      out[0] = *reinterpret_cast<const float2*>(q);
+    } else {
+      out[0] = *q;
     }
   }
 }
-template <typename T, int V>
-__device__ __forceinline__ Pack<T, V> head_pack(const float (&f)[V]) {
-  typename MathSel<V>::M::E lanes[MathSel<V>::NE];
-  if constexpr (V == 1) {
-    lanes[0] = f[0];
-  } else {
+template <int V>
+__device__ __forceinline__ void head_sums_store(float* p, int j, const typename MathSel<V>::M::E (&in)[MathSel<V>::NE]) {
+  constexpr int CW = HeadTraits<V>::CW;
 #pragma unroll
-    for (int i = 0; i < V / 2; ++i) lanes[i] = make_float2(f[2 * i], f[2 * i + 1]);
+  for (int c = 0; c < V / CW; ++c) {
+    float* q = p + (j * (V / CW) + c) * CW * kHeadBlock;
+    if constexpr (CW == 4) {
+      *reinterpret_cast<float4*>(q) = make_float4(in[2 * c].x, in[2 * c].y, in[2 * c + 1].x, in[2 * c + 1].y);
+    } else if constexpr (CW == 2) {
+      *reinterpret_cast<float2*>(q) = in[0];
+    } else {
+      *q = in[0];
+    }
   }
-  return repack<T, V>(lanes);
+}
+
+// Turns every slot of a row by its token's angles.
+template <int V, bool IL, int SIGN, int SPT, typename E, int NE>
+__device__ __forceinline__ void head_rotate(E (&v)[SPT][2][NE], const float* tab, int lane, int tph,
+                                            const bool (&rot)[SPT][2]) {
+#pragma unroll
+  for (int i = 0; i < SPT; ++i) {
+    float c[V], s[V];
+    head_table_read<V>(tab, false, lane + i * tph, SPT * tph, c);
+    head_table_read<V>(tab, true, lane + i * tph, SPT * tph, s);
+    head_turn<V, IL, SIGN>(v[i][0], v[i][1], c, s, rot[i][0], rot[i][1]);
+  }
 }
 
 // NORM: 0 none, 1 root mean square, 2 mean and variance.  IL: interleaved pairs.
 template <typename T, int V, int NORM, bool IL, bool BWD>
-__global__ void __launch_bounds__(kHeadBlock) head_kernel(const HeadArgs a) {
-  constexpr int SPT = HeadTraits<T, V>::SPT;
+__global__ void __launch_bounds__(kHeadBlock, BWD ? 2 : 3) head_kernel(const HeadArgs a) {
+  constexpr int SPT = HeadTraits<V>::SPT;
+  using M = typename MathSel<V>::M;
+  using E = typename M::E;
+  constexpr int NE = MathSel<V>::NE;
   using P = Pack<T, V>;
-  constexpr int R = (BWD ? 2 : 4) / (sizeof(T) == 4 ? 2 : 1);   // rows in flight per group
-  constexpr int NV = NORM == 0 ? 0 : (NORM == 1 ? 1 : 2);       // parameter vectors per part
-  // dynamic shared memory: cos [tile][pstride], sin [tile][pstride], parameters [2][NV][hd4],
-  // gradient sums [2][NV][16][kHeadBlock] (backward)
+  constexpr int NV = NORM;                         // parameter vectors per part
+  constexpr bool READ_X = !BWD || NORM != 0;       // without a norm the gradient needs no x
+  constexpr int OFFS = BWD ? 3 : 2;                // tensors with offsets: out, x, dy
+  // dynamic shared memory: gradient sums [2][NV][16][kHeadBlock] (backward), parameters
+  // [2][NV][hd4], three buffers of angles [tile][pstride] and of offsets [2][OFFS][tile]
   extern __shared__ __align__(16) float head_smem[];
-  float* const cos_t = head_smem;
-  float* const sin_t = cos_t + a.tile * a.pstride;
-  float* const par = sin_t + a.tile * a.pstride;
-  float* const sums = par + 2 * NV * a.hd4;
+  float* const sums = head_smem;
+  float* const par = head_smem + (BWD ? 2 * NV * 16 * kHeadBlock : 0);
+  float* const tables = par + 2 * NV * a.hd4;
+  const int table_floats = a.tile * a.pstride;
+  int64_t* const offsets = reinterpret_cast<int64_t*>(tables + 3 * table_floats);
+  const int buffer_offsets = 2 * OFFS * a.tile;
 
   const int tid = threadIdx.x;
   const int tph = a.tph;
   const int lane = tid & (tph - 1);
   const int group = tid / tph;
   const int groups = kHeadBlock / tph;
+  const int nslots = SPT * tph;
   const int pairs = a.pairs;
   const int vectors = a.hd / V;
 
@@ -158,6 +248,12 @@ __global__ void __launch_bounds__(kHeadBlock) head_kernel(const HeadArgs a) {
       const float* src = NV == 1 ? a.param[2 * which] : a.param[which];
       par[i] = src != nullptr && col < a.hd ? __ldg(src + col) : 0.f;
     }
+  }
+  // slots behind the rotated pairs turn by nothing
+  for (int i = tid; i < 3 * a.tile * (nslots * V - pairs); i += kHeadBlock) {
+    const int row = i / (nslots * V - pairs), p = pairs + i - row * (nslots * V - pairs);
+    tables[row * a.pstride + head_table_at<V>(p, false, nslots)] = 1.f;
+    tables[row * a.pstride + head_table_at<V>(p, true, nslots)] = 0.f;
   }
 
   // this thread's vectors
@@ -174,51 +270,29 @@ __global__ void __launch_bounds__(kHeadBlock) head_kernel(const HeadArgs a) {
     }
   }
 
-  P xr[R][SPT][2], dr[BWD ? R : 1][SPT][2];
-  // Row `u` of a part's tile: its token in the tile and its element offsets.
-  auto fetch = [&](int part, int64_t n0, int base, int rows) {
-    const HeadPart& hp = a.part[part];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int u = base + r * groups + group;
-      const bool on = u < rows;
-      const unsigned lt = fast_div(static_cast<unsigned>(u), hp.div);
-      const int64_t h = u - static_cast<int>(lt) * hp.heads;
-      const unsigned n = static_cast<unsigned>(n0) + lt;
-      const unsigned b = fast_div(n, a.tdiv);
-      const int64_t t = n - b * static_cast<unsigned>(a.T);
-      const T* xp = static_cast<const T*>(hp.x) + (b * hp.xs[0] + t * hp.xs[1] + h * hp.xs[2]);
-      const T* dp = static_cast<const T*>(hp.dy);
-      if constexpr (BWD) dp += b * hp.ds[0] + t * hp.ds[1] + h * hp.ds[2];
-#pragma unroll
-      for (int i = 0; i < SPT; ++i)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          if (on && valid[i][k]) {
-            if (!BWD || NORM != 0) xr[r][i][k] = load_stream<T, V>(xp, col[i][k]);
-            if constexpr (BWD) dr[r][i][k] = load_stream<T, V>(dp, col[i][k]);
-          } else {
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-              xr[r][i][k].v[e] = Cvt<T>::from_f32(0.f);
-              if constexpr (BWD) dr[r][i][k].v[e] = Cvt<T>::from_f32(0.f);
-            }
-          }
-        }
-    }
+  auto tokens_of = [&](int64_t tile) {
+    const int64_t left = a.N - tile * a.tile;
+    return static_cast<int>(left < a.tile ? left : a.tile);
   };
-
-  bool first = true;
-  for (int64_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
-    const int64_t n0 = tile * a.tile;
-    const int tokens = static_cast<int>(a.N - n0 < a.tile ? a.N - n0 : a.tile);
-    fetch(0, n0, 0, tokens * a.part[0].heads);
-    // the angles of the tile's tokens
-    if (!first) __syncthreads();   // everybody is past the previous tile's table
+  // The tables of a tile: angles, and where each token's rows begin.
+  auto make_tables = [&](int64_t tile, int buf) {
+    const unsigned n0 = static_cast<unsigned>(tile * a.tile);
+    const int tokens = tokens_of(tile);
+    float* tab = tables + buf * table_floats;
+    int64_t* off = offsets + buf * buffer_offsets;
+    for (int i = tid; i < tokens * a.parts; i += kHeadBlock) {
+      const int part = i >= tokens ? 1 : 0, lt = i - part * tokens;
+      const HeadPart& hp = a.part[part];
+      const unsigned n = n0 + lt, b = fast_div(n, a.tdiv);
+      const int64_t t = n - b * static_cast<unsigned>(a.T);
+      int64_t* o = off + part * OFFS * a.tile + lt;
+      o[0] = b * hp.os[0] + t * hp.os[1];
+      o[a.tile] = b * hp.xs[0] + t * hp.xs[1];
+      if constexpr (BWD) o[2 * a.tile] = b * hp.ds[0] + t * hp.ds[1];
+    }
     for (int i = tid; i < tokens * pairs; i += kHeadBlock) {
-      const int lt = i / pairs, p = i - lt * pairs;
-      const unsigned n = static_cast<unsigned>(n0) + lt;
-      const unsigned b = fast_div(n, a.tdiv);
+      const int lt = static_cast<int>(fast_div(static_cast<unsigned>(i), a.pdiv)), p = i - lt * pairs;
+      const unsigned n = n0 + lt, b = fast_div(n, a.tdiv);
       const int64_t t = n - b * static_cast<unsigned>(a.T);
       const int axis = __ldg(a.pair_axis + p);
       float c = 1.f, s = 0.f;
@@ -230,185 +304,223 @@ __global__ void __launch_bounds__(kHeadBlock) head_kernel(const HeadArgs a) {
         turns -= rint(turns);
         sincospif(2.f * static_cast<float>(turns), &s, &c);
       }
-      cos_t[lt * a.pstride + p] = c;
-      sin_t[lt * a.pstride + p] = s;
+      tab[lt * a.pstride + head_table_at<V>(p, false, nslots)] = c;
+      tab[lt * a.pstride + head_table_at<V>(p, true, nslots)] = s;
     }
-    __syncthreads();
+  };
 
-#pragma unroll 1
-    for (int part = 0; part < a.parts; ++part) {
-      const HeadPart& hp = a.part[part];
-      const int rows = tokens * hp.heads;
-      float g[SPT][2][V], off[SPT][2][V];
-      float dg[SPT][2][V], db[SPT][2][V];
+  P xr[SPT][2], dr[SPT][2];
+  auto clear = [&]() {
+#pragma unroll
+    for (int i = 0; i < SPT; ++i)
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int e = 0; e < V; ++e) xr[i][k].v[e] = dr[i][k].v[e] = Cvt<T>::from_f32(0.f);
+  };
+  // Starts the loads of row `base + group` of a part's tile.
+  auto fetch = [&](int part, int buf, int base, int rows) {
+    const HeadPart& hp = a.part[part];
+    const int u = base + group;
+    if (u < rows) {
+      const unsigned lt = fast_div(static_cast<unsigned>(u), hp.div);
+      const int64_t h = u - static_cast<int>(lt) * hp.heads;
+      const int64_t* o = offsets + buf * buffer_offsets + part * OFFS * a.tile + lt;
+      const T* xp = static_cast<const T*>(hp.x) + o[a.tile] + h * hp.xs[2];
+      const T* dp = nullptr;
+      if constexpr (BWD) dp = static_cast<const T*>(hp.dy) + o[2 * a.tile] + h * hp.ds[2];
 #pragma unroll
       for (int i = 0; i < SPT; ++i)
 #pragma unroll
         for (int k = 0; k < 2; ++k)
+          if (valid[i][k]) {
+            if constexpr (READ_X) xr[i][k] = load_stream<T, V>(xp, col[i][k]);
+            if constexpr (BWD) dr[i][k] = load_stream<T, V>(dp, col[i][k]);
+          }
+    } else if constexpr (BWD) {
+      clear();   // a group without a row adds nothing to the parameter sums
+    }
+  };
+  clear();
+
+  const int64_t tile0 = blockIdx.x;
+  make_tables(tile0, 0);
+  __syncthreads();
+  fetch(0, 0, 0, tokens_of(tile0) * a.part[0].heads);
+  int buf = 0;
+  for (int64_t tile = tile0; tile < a.tiles; tile += gridDim.x) {
+    const bool more = tile + gridDim.x < a.tiles;
+    const int next_buf = buf == 2 ? 0 : buf + 1;
+    if (more) make_tables(tile + gridDim.x, next_buf);
+    if (tile != tile0 || more) __syncthreads();
+    const int tokens = tokens_of(tile);
+    const float* tab = tables + buf * table_floats;
+    const int64_t* off = offsets + buf * buffer_offsets;
+#pragma unroll 1
+    for (int part = 0; part < a.parts; ++part) {
+      const HeadPart& hp = a.part[part];
+      const int rows = tokens * hp.heads;
+      E g[SPT][2][NE], dg[SPT][2][NE], db[SPT][2][NE];
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const float* pv = par + part * NV * a.hd4 + (valid[i][k] ? col[i][k] + e : 0);
-            if constexpr (NORM != 0) g[i][k][e] = pv[0];
-            if constexpr (NORM == 2 && !BWD) off[i][k][e] = pv[a.hd4];
-            if constexpr (BWD && NORM != 0) {
-              const float* sv = sums + (part * NV * 16 + (i * 2 + k) * V + e) * kHeadBlock + tid;
-              dg[i][k][e] = first ? 0.f : sv[0];
-              if constexpr (NORM == 2) db[i][k][e] = first ? 0.f : sv[16 * kHeadBlock];
+      for (int i = 0; i < SPT; ++i)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          if constexpr (NORM != 0)
+            head_lanes<V>(par + part * NV * a.hd4 + (valid[i][k] ? col[i][k] : 0), g[i][k]);
+        }
+      float* const mine = sums + part * NV * 16 * kHeadBlock + tid * HeadTraits<V>::CW;
+      if constexpr (BWD && NORM != 0) {
+#pragma unroll
+        for (int i = 0; i < SPT; ++i)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            if (tile != tile0) {
+              head_sums_load<V>(mine, i * 2 + k, dg[i][k]);
+              if constexpr (NORM == 2) head_sums_load<V>(mine + 16 * kHeadBlock, i * 2 + k, db[i][k]);
+            } else {
+#pragma unroll
+              for (int e = 0; e < NE; ++e) dg[i][k][e] = db[i][k][e] = M::bcast(0.f);
             }
           }
-      for (int base = 0; base < rows; base += groups * R) {
-        if (part > 0 || base > 0) fetch(part, n0, base, rows);
+      }
+#pragma unroll 1
+      for (int base = 0; base < rows; base += groups) {
+        E x[SPT][2][NE], d[SPT][2][NE];
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-          const int u = base + r * groups + group;
-          const bool on = u < rows;
-          const unsigned lt = on ? fast_div(static_cast<unsigned>(u), hp.div) : 0;
-          const float* ct = cos_t + lt * a.pstride;
-          const float* st = sin_t + lt * a.pstride;
-          float x[SPT][2][V], d[SPT][2][V];
+        for (int i = 0; i < SPT; ++i)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            if constexpr (READ_X) unpack<T, V>(xr[i][k], x[i][k]);
+            if constexpr (BWD) unpack<T, V>(dr[i][k], d[i][k]);
+          }
+        {  // the group's next row
+          int nb = base + groups, np = part;
+          bool nt = false;
+          if (nb >= rows) {
+            nb = 0;
+            if (++np == a.parts) np = 0, nt = true;
+          }
+          if (!nt) {
+            fetch(np, buf, nb, tokens * a.part[np].heads);
+          } else if (more) {
+            fetch(0, next_buf, 0, tokens_of(tile + gridDim.x) * a.part[0].heads);
+          }
+        }
+        const int u = base + group;
+        const bool on = u < rows;
+        const unsigned lt = on ? fast_div(static_cast<unsigned>(u), hp.div) : 0;
+        const float* tt = tab + lt * a.pstride;
+        if constexpr (BWD) head_rotate<V, IL, -1>(d, tt, lane, tph, rot);
+        if constexpr (NORM == 2) {
+          E acc = M::bcast(0.f);
 #pragma unroll
           for (int i = 0; i < SPT; ++i)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              head_unpack<T, V>(xr[r][i][k], x[i][k]);
-              if constexpr (BWD) head_unpack<T, V>(dr[r][i][k], d[i][k]);
-            }
-          float inv = 1.f;
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+              for (int e = 0; e < NE; ++e) acc = M::add(acc, x[i][k][e]);
+          float m[1] = {M::hsum(acc)};
+          head_reduce<1>(m, tph);
+          const E nm = M::bcast(-m[0] * a.inv_hd);
+#pragma unroll
+          for (int i = 0; i < SPT; ++i)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+              for (int e = 0; e < NE; ++e) x[i][k][e] = valid[i][k] ? M::add(x[i][k][e], nm) : M::bcast(0.f);
+        }
+        if constexpr (NORM != 0) {
+          // sum of squares; backward: sum gy c and, for mean and variance, sum gy beside it
+          constexpr int NR = BWD ? NORM + 1 : 1;
+          E acc[NR];
+#pragma unroll
+          for (int k = 0; k < NR; ++k) acc[k] = M::bcast(0.f);
+#pragma unroll
+          for (int i = 0; i < SPT; ++i)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+              for (int e = 0; e < NE; ++e) {
+                acc[0] = M::fma(x[i][k][e], x[i][k][e], acc[0]);
+                if constexpr (BWD) {
+                  const E gy = M::mul(d[i][k][e], g[i][k][e]);
+                  acc[1] = M::fma(gy, x[i][k][e], acc[1]);
+                  if constexpr (NORM == 2) acc[NORM] = M::add(acc[NORM], gy);
+                }
+              }
+          float red[NR];
+#pragma unroll
+          for (int k = 0; k < NR; ++k) red[k] = M::hsum(acc[k]) * a.inv_hd;  // shares of means: no overflow in the sum
+          head_reduce<NR>(red, tph);
+          // a group without a row must not put 0 * inf into the parameter sums
+          const float inv = on ? rsqrtf(red[0] + a.eps) : 0.f;
+          const E iv = M::bcast(inv);
           if constexpr (BWD) {
-#pragma unroll
-            for (int i = 0; i < SPT; ++i) {
-              const int p0 = (lane + i * tph) * V;
-              float c[V], s[V];
-#pragma unroll
-              for (int e = 0; e < V; ++e) {
-                const bool in = p0 + e < pairs;
-                c[e] = in ? ct[p0 + e] : 1.f;
-                s[e] = in ? st[p0 + e] : 0.f;
-              }
-              head_turn<V, IL, -1>(d[i][0], d[i][1], c, s, rot[i][0], rot[i][1]);
-            }
-          }
-          if constexpr (NORM == 2) {
-            float m[1] = {0.f};
+            const E nm1 = M::bcast(-red[1] * inv);
+            const E nm0 = M::bcast(NORM == 2 ? -red[NORM] : 0.f);
 #pragma unroll
             for (int i = 0; i < SPT; ++i)
 #pragma unroll
               for (int k = 0; k < 2; ++k)
 #pragma unroll
-                for (int e = 0; e < V; ++e) m[0] += x[i][k][e];
-            head_reduce<1>(m, tph);
-            m[0] *= a.inv_hd;
-#pragma unroll
-            for (int i = 0; i < SPT; ++i)
-#pragma unroll
-              for (int k = 0; k < 2; ++k)
-#pragma unroll
-                for (int e = 0; e < V; ++e) x[i][k][e] = valid[i][k] ? x[i][k][e] - m[0] : 0.f;
-          }
-          if constexpr (NORM != 0) {
-            // sum of squares; backward: sum gy c and, for mean and variance, sum gy beside it
-            constexpr int NR = BWD ? NORM + 1 : 1;
-            float red[NR];
-#pragma unroll
-            for (int k = 0; k < NR; ++k) red[k] = 0.f;
-#pragma unroll
-            for (int i = 0; i < SPT; ++i)
-#pragma unroll
-              for (int k = 0; k < 2; ++k)
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                  red[0] = fmaf(x[i][k][e], x[i][k][e], red[0]);
-                  if constexpr (BWD) {
-                    const float gy = d[i][k][e] * g[i][k][e];
-                    red[1] = fmaf(gy, x[i][k][e], red[1]);
-                    if constexpr (NORM == 2) red[2] += gy;
-                  }
+                for (int e = 0; e < NE; ++e) {
+                  const E xh = M::mul(x[i][k][e], iv);
+                  dg[i][k][e] = M::fma(d[i][k][e], xh, dg[i][k][e]);
+                  if constexpr (NORM == 2) db[i][k][e] = M::add(db[i][k][e], d[i][k][e]);
+                  const E gy = NORM == 2 ? M::fma(d[i][k][e], g[i][k][e], nm0) : M::mul(d[i][k][e], g[i][k][e]);
+                  d[i][k][e] = M::mul(M::fma(nm1, xh, gy), iv);
                 }
-#pragma unroll
-            for (int k = 0; k < NR; ++k) red[k] *= a.inv_hd;   // shares of means: no overflow in the sum
-            head_reduce<NR>(red, tph);
-            // a group without a row must not put 0 * inf into the parameter sums
-            inv = on ? rsqrtf(red[0] + a.eps) : 0.f;
-            if constexpr (BWD) {
-              const float m1 = red[1] * inv;
-              const float m0 = NORM == 2 ? red[NORM] : 0.f;
-#pragma unroll
-              for (int i = 0; i < SPT; ++i)
-#pragma unroll
-                for (int k = 0; k < 2; ++k)
-#pragma unroll
-                  for (int e = 0; e < V; ++e) {
-                    const float xh = x[i][k][e] * inv;
-                    dg[i][k][e] = fmaf(d[i][k][e], xh, dg[i][k][e]);
-                    if constexpr (NORM == 2) db[i][k][e] += d[i][k][e];
-                    const float gy = fmaf(d[i][k][e], g[i][k][e], -m0);
-                    d[i][k][e] = fmaf(-m1, xh, gy) * inv;
-                  }
-            } else {
-#pragma unroll
-              for (int i = 0; i < SPT; ++i)
-#pragma unroll
-                for (int k = 0; k < 2; ++k)
-#pragma unroll
-                  for (int e = 0; e < V; ++e)
-                    x[i][k][e] = NORM == 2 ? fmaf(x[i][k][e] * inv, g[i][k][e], off[i][k][e])
-                                           : x[i][k][e] * inv * g[i][k][e];
-            }
-          }
-          if constexpr (!BWD) {
-#pragma unroll
-            for (int i = 0; i < SPT; ++i) {
-              const int p0 = (lane + i * tph) * V;
-              float c[V], s[V];
-#pragma unroll
-              for (int e = 0; e < V; ++e) {
-                const bool in = p0 + e < pairs;
-                c[e] = in ? ct[p0 + e] : 1.f;
-                s[e] = in ? st[p0 + e] : 0.f;
-              }
-              head_turn<V, IL, 1>(x[i][0], x[i][1], c, s, rot[i][0], rot[i][1]);
-            }
-          }
-          if (on) {
-            const int64_t h = u - static_cast<int>(lt) * hp.heads;
-            const unsigned n = static_cast<unsigned>(n0) + lt;
-            const unsigned b = fast_div(n, a.tdiv);
-            const int64_t t = n - b * static_cast<unsigned>(a.T);
-            T* op = static_cast<T*>(hp.out) + (b * hp.os[0] + t * hp.os[1] + h * hp.os[2]);
+          } else {
 #pragma unroll
             for (int i = 0; i < SPT; ++i)
 #pragma unroll
-              for (int k = 0; k < 2; ++k)
-                if (valid[i][k]) {
-                  if constexpr (BWD) {
-                    store_stream<T, V>(op, col[i][k], head_pack<T, V>(d[i][k]));
-                  } else {
-                    store_stream<T, V>(op, col[i][k], head_pack<T, V>(x[i][k]));
-                  }
+              for (int k = 0; k < 2; ++k) {
+                E be[NE];   // the offsets stay in shared memory: registers are short here
+                if constexpr (NORM == 2)
+                  head_lanes<V>(par + (part * NV + 1) * a.hd4 + (valid[i][k] ? col[i][k] : 0), be);
+#pragma unroll
+                for (int e = 0; e < NE; ++e) {
+                  const E xh = M::mul(x[i][k][e], iv);
+                  x[i][k][e] = NORM == 2 ? M::fma(xh, g[i][k][e], be[e]) : M::mul(xh, g[i][k][e]);
                 }
+              }
           }
+        }
+        if constexpr (!BWD) head_rotate<V, IL, 1>(x, tt, lane, tph, rot);
+        if (on) {
+          const int64_t h = u - static_cast<int>(lt) * hp.heads;
+          T* op = static_cast<T*>(hp.out) + off[part * OFFS * a.tile + lt] + h * hp.os[2];
+#pragma unroll
+          for (int i = 0; i < SPT; ++i)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              if (valid[i][k]) {
+                if constexpr (BWD) {
+                  store_stream<T, V>(op, col[i][k], repack<T, V>(d[i][k]));
+                } else {
+                  store_stream<T, V>(op, col[i][k], repack<T, V>(x[i][k]));
+                }
+              }
         }
       }
       if constexpr (BWD && NORM != 0) {
 #pragma unroll
         for (int i = 0; i < SPT; ++i)
 #pragma unroll
-          for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-              float* sv = sums + (part * NV * 16 + (i * 2 + k) * V + e) * kHeadBlock + tid;
-              sv[0] = dg[i][k][e];
-              if constexpr (NORM == 2) sv[16 * kHeadBlock] = db[i][k][e];
-            }
+          for (int k = 0; k < 2; ++k) {
+            head_sums_store<V>(mine, i * 2 + k, dg[i][k]);
+            if constexpr (NORM == 2) head_sums_store<V>(mine + 16 * kHeadBlock, i * 2 + k, db[i][k]);
+          }
       }
     }
-    first = false;
+    buf = next_buf;
   }
 
   if constexpr (BWD && NORM != 0) {
     // the CTA's sums of the groups, in group order: one partial row [parts][NV][hd]
     __syncthreads();
     float* w = a.ws + static_cast<int64_t>(blockIdx.x) * a.parts * NV * a.hd;
+    constexpr int CW = HeadTraits<V>::CW;
     for (int o = tid; o < a.parts * NV * 16 * tph; o += kHeadBlock) {
       const int vec = o / (16 * tph), rest = o - vec * 16 * tph;
       const int el = rest / tph, ln = rest - el * tph;
@@ -416,7 +528,8 @@ __global__ void __launch_bounds__(kHeadBlock) head_kernel(const HeadArgs a) {
       const bool in = (!IL && s * V < pairs) || 2 * s + half < vectors;
       if (!in) continue;
       float t = 0.f;
-      for (int gr = 0; gr < groups; ++gr) t += sums[(vec * 16 + el) * kHeadBlock + gr * tph + ln];
+      for (int gr = 0; gr < groups; ++gr)
+        t += sums[(vec * 16 + el / CW * CW) * kHeadBlock + (gr * tph + ln) * CW + el % CW];
       w[vec * a.hd + head_col<V, IL>(s, half, pairs) + el % V] = t;
     }
   }

@@ -27,56 +27,53 @@ namespace nvn {
 namespace {
 
 constexpr bool kBwd = NVN_BWD != 0;
-constexpr int kTableBytes = 32 * 1024;   // most a tile's cosines and sines may take
+constexpr int kTableBytes = 48 * 1024;   // most that a CTA's tables may take
 
 inline int round4(int v) { return (v + 3) / 4 * 4; }
 
 template <int V, int NORM, bool IL>
 cudaError_t launch(HeadArgs& a, cudaStream_t s, bool dry_run, HeadPlan* plan) {
   auto kernel = head_kernel<T, V, NORM, IL, kBwd>;
-  constexpr int SPT = HeadTraits<T, V>::SPT;
-  constexpr int NV = NORM == 0 ? 0 : (NORM == 1 ? 1 : 2);
-  constexpr int R = (kBwd ? 2 : 4) / (sizeof(T) == 4 ? 2 : 1);
+  constexpr int SPT = HeadTraits<V>::SPT;
+  constexpr int NV = NORM;
   const int slots = (a.hd + 2 * V - 1) / (2 * V);
   a.tph = 1;
   while (a.tph * SPT < slots) a.tph *= 2;
   if (a.tph > 32) return cudaErrorInvalidValue;
-  a.pstride = round4(a.pairs > 0 ? a.pairs : 1);
+  a.pstride = a.tph * SPT * V * 2;
   a.hd4 = round4(a.hd);
-  // A tile holds two batches of rows for every group, less when that leaves SMs without a CTA.
+  // A tile holds eight rows for every group, less when that leaves SMs without a CTA.
   const int heads = a.part[0].heads + (a.parts > 1 ? a.part[1].heads : 0);
   const int groups = kHeadBlock / a.tph;
-  int64_t tile = heads > 0 ? (2 * R * groups + heads - 1) / heads : 1;
+  int64_t tile = heads > 0 ? (8 * groups + heads - 1) / heads : 1;
   const int64_t spread = a.N / (static_cast<int64_t>(device_sm_count()) * 4);
   if (tile > spread) tile = spread;
-  const int64_t most = kTableBytes / (8 * a.pstride);
-  if (tile > most) tile = most;
+  const int token_bytes = 3 * (a.pstride * 4 + 2 * (kBwd ? 3 : 2) * 8);
+  if (tile > kTableBytes / token_bytes) tile = kTableBytes / token_bytes;
   a.tile = static_cast<int>(tile < 1 ? 1 : tile);
   a.tiles = (a.N + a.tile - 1) / a.tile;
-  const size_t smem = (static_cast<size_t>(2) * a.tile * a.pstride + 2 * NV * a.hd4 +
-                       (kBwd ? 2 * NV * 16 * kHeadBlock : 0)) * 4;
+  const size_t fixed = static_cast<size_t>(2 * NV * a.hd4 + (kBwd ? 2 * NV * 16 * kHeadBlock : 0)) * 4;
+  const size_t smem = fixed + static_cast<size_t>(a.tile) * token_bytes;
   static std::atomic<uint64_t> prepared{0};
   cudaError_t e = once_per_device(prepared, [&]() -> cudaError_t {
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                 kTableBytes + (2 * NV * 512 + (kBwd ? 2 * NV * 16 * kHeadBlock : 0)) * 4);
   });
   if (e != cudaSuccess) return e;
-  int64_t grid = a.tiles;
-  if (kBwd) {   // persistent: the parameter sums stay in the CTA over all its tiles
-    static std::atomic<int64_t> cached{0};  // (shared bytes << 20) | CTAs per SM
-    const int64_t c = cached.load(std::memory_order_relaxed);
-    int per_sm = 0;
-    if (c != 0 && static_cast<size_t>(c >> 20) == smem) {
-      per_sm = static_cast<int>(c & 0xfffff);
-    } else {
-      e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kHeadBlock, smem);
-      if (e != cudaSuccess) return e;
-      if (per_sm < 1) per_sm = 1;
-      cached.store((static_cast<int64_t>(smem) << 20) | per_sm, std::memory_order_relaxed);
-    }
-    const int64_t resident = static_cast<int64_t>(per_sm) * device_sm_count();
-    if (grid > resident) grid = resident;
+  // persistent: tables and (backward) the parameter sums of a CTA serve all its tiles
+  static std::atomic<int64_t> cached{0};  // (shared bytes << 20) | CTAs per SM
+  const int64_t c = cached.load(std::memory_order_relaxed);
+  int per_sm = 0;
+  if (c != 0 && static_cast<size_t>(c >> 20) == smem) {
+    per_sm = static_cast<int>(c & 0xfffff);
+  } else {
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kHeadBlock, smem);
+    if (e != cudaSuccess) return e;
+    if (per_sm < 1) per_sm = 1;
+    cached.store((static_cast<int64_t>(smem) << 20) | per_sm, std::memory_order_relaxed);
   }
+  const int64_t resident = static_cast<int64_t>(per_sm) * device_sm_count();
+  const int64_t grid = a.tiles < resident ? a.tiles : resident;
   plan->v = V;
   plan->grid = static_cast<int>(grid);
   plan->smem = smem;

@@ -333,7 +333,7 @@ struct HeadArgs {
   int64_t ps[3];          // strides of positions: axis, batch, token
   int pos64, axes, pairs;
   int64_t N, T, tiles;    // N = batch * tokens
-  HeadDiv tdiv;           // by T
+  HeadDiv tdiv, pdiv;     // by T, by pairs
   int hd, hd4, tph, tile, pstride;
   float inv_hd, eps;
 };
