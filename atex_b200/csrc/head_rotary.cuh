@@ -20,15 +20,17 @@
 //   behind the rotated elements a slot is 2V plain elements.
 // In every form slot s turns by the V angles from pair sV on.
 //
-// A CTA takes tiles of consecutive tokens with all their heads, queries and keys: the angles of a
-// token are the same for all of them and are computed once per tile into shared memory - in 64
+// A CTA takes tiles: a block of consecutive tokens with all their heads, queries and keys - or, when
+// a token has more rows than a tile, or tokens are few, a piece of the block's rows.  The angles of a
+// token are the same for all its heads and are computed once per tile into shared memory - in 64
 // bits up to the fraction of a turn, because a position of a million times a frequency has no
-// fraction left in 32.  The rows of a tile are dealt to the groups of TPH lanes; while a group
-// works on a row its next one is already on the way into registers, across the ends of parts and
-// tiles too.  The tables (angles, and the element offsets of the tokens) have three buffers, so
-// that one barrier per tile is enough: tile i reads buffer i, its last rows fetch from the offsets
-// of buffer i + 1, and the barrier in tile i + 1 stands between the last read of buffer i and its
-// refill in tile i + 2.
+// fraction left in 32.  Where each row of a tile begins is worked out once as well, by one thread a
+// row: done by every lane for every row it was two thirds of the instructions.  The rows of a tile
+// are dealt to the groups of TPH lanes; while a group works on a row its next one is already on the
+// way into registers, across the ends of parts and tiles too.  The tables (angles, row addresses)
+// have three buffers, so that one barrier per tile is enough: tile i reads buffer i, its last rows
+// fetch from the addresses of buffer i + 1, and the barrier in tile i + 1 stands between the last
+// read of buffer i and its refill in tile i + 2.
 #pragma once
 
 #include "nvn_common.cuh"
@@ -210,6 +212,17 @@ __device__ __forceinline__ void head_rotate(E (&v)[SPT][2][NE], const float* tab
   }
 }
 
+// Where a row is read, and where it goes: null for a row that is none.
+struct alignas(16) HeadSource {
+  const void* x;
+  const void* dy;
+};
+struct alignas(16) HeadTarget {
+  void* out;
+  int angles;   // of the row's token, in the tile's table
+  int unused;
+};
+
 // NORM: 0 none, 1 root mean square, 2 mean and variance.  IL: interleaved pairs.
 template <typename T, int V, int NORM, bool IL, bool BWD>
 __global__ void __launch_bounds__(kHeadBlock, BWD ? 2 : 3) head_kernel(const HeadArgs a) {
@@ -220,22 +233,23 @@ __global__ void __launch_bounds__(kHeadBlock, BWD ? 2 : 3) head_kernel(const Hea
   using P = Pack<T, V>;
   constexpr int NV = NORM;                         // parameter vectors per part
   constexpr bool READ_X = !BWD || NORM != 0;       // without a norm the gradient needs no x
-  constexpr int OFFS = BWD ? 3 : 2;                // tensors with offsets: out, x, dy
-  // dynamic shared memory: gradient sums [2][NV][16][kHeadBlock] (backward), parameters
-  // [2][NV][hd4], three buffers of angles [tile][pstride] and of offsets [2][OFFS][tile]
+  // dynamic shared memory: gradient sums [2][NV][16][kHeadBlock] (backward), three buffers of row
+  // addresses [rows] (where x and dy are read; where the result goes, and the row's angles),
+  // parameters [2][NV][hd4], three buffers of angles [tile][pstride]
   extern __shared__ __align__(16) float head_smem[];
   float* const sums = head_smem;
-  float* const par = head_smem + (BWD ? 2 * NV * 16 * kHeadBlock : 0);
+  HeadSource* const sources = reinterpret_cast<HeadSource*>(sums + (BWD ? 2 * NV * 16 * kHeadBlock : 0));
+  HeadTarget* const targets = reinterpret_cast<HeadTarget*>(sources + 3 * a.rows);
+  float* const par = reinterpret_cast<float*>(targets + 3 * a.rows);
   float* const tables = par + 2 * NV * a.hd4;
   const int table_floats = a.tile * a.pstride;
-  int64_t* const offsets = reinterpret_cast<int64_t*>(tables + 3 * table_floats);
-  const int buffer_offsets = 2 * OFFS * a.tile;
 
   const int tid = threadIdx.x;
   const int tph = a.tph;
   const int lane = tid & (tph - 1);
   const int group = tid / tph;
   const int groups = kHeadBlock / tph;
+  const int glog = 31 - __clz(groups);
   const int nslots = SPT * tph;
   const int pairs = a.pairs;
   const int vectors = a.hd / V;
@@ -270,25 +284,49 @@ __global__ void __launch_bounds__(kHeadBlock, BWD ? 2 : 3) head_kernel(const Hea
     }
   }
 
-  auto tokens_of = [&](int64_t tile) {
-    const int64_t left = a.N - tile * a.tile;
-    return static_cast<int>(left < a.tile ? left : a.tile);
+  if constexpr (BWD && NORM != 0) {
+    for (int i = tid; i < 2 * NV * 16 * kHeadBlock; i += kHeadBlock) sums[i] = 0.f;
+  }
+
+  // A tile's block of tokens and its first step (a step is one row for every group).
+  auto place = [&](int64_t tile, int64_t& block, int& first) {
+    block = tile;
+    first = 0;
+    if (a.pieces > 1) {
+      block = tile / a.pieces;
+      first = static_cast<int>(tile - block * a.pieces) * a.steps;
+    }
   };
-  // The tables of a tile: angles, and where each token's rows begin.
+  // The tables of a tile: angles, and where each row begins (nowhere for the rows that fill up a
+  // part's last step or lie behind the last token).
   auto make_tables = [&](int64_t tile, int buf) {
-    const unsigned n0 = static_cast<unsigned>(tile * a.tile);
-    const int tokens = tokens_of(tile);
+    int64_t block;
+    int first;
+    place(tile, block, first);
+    const int64_t left = a.N - block * a.tile;
+    const int tokens = static_cast<int>(left < a.tile ? left : a.tile);
+    const unsigned n0 = static_cast<unsigned>(block * a.tile);
     float* tab = tables + buf * table_floats;
-    int64_t* off = offsets + buf * buffer_offsets;
-    for (int i = tid; i < tokens * a.parts; i += kHeadBlock) {
-      const int part = i >= tokens ? 1 : 0, lt = i - part * tokens;
+    const int steps = a.all_steps - first < a.steps ? a.all_steps - first : a.steps;
+    for (int i = tid; i < steps * groups; i += kHeadBlock) {
+      const int step = first + (i >> glog);
+      const int part = step >= a.q_steps ? 1 : 0;
       const HeadPart& hp = a.part[part];
-      const unsigned n = n0 + lt, b = fast_div(n, a.tdiv);
-      const int64_t t = n - b * static_cast<unsigned>(a.T);
-      int64_t* o = off + part * OFFS * a.tile + lt;
-      o[0] = b * hp.os[0] + t * hp.os[1];
-      o[a.tile] = b * hp.xs[0] + t * hp.xs[1];
-      if constexpr (BWD) o[2 * a.tile] = b * hp.ds[0] + t * hp.ds[1];
+      const int u = i + ((first - (part ? a.q_steps : 0)) << glog);
+      const int lt = static_cast<int>(fast_div(static_cast<unsigned>(u), hp.div));
+      HeadSource src = {nullptr, nullptr};
+      HeadTarget dst = {nullptr, 0, 0};
+      if (lt < tokens) {
+        const int64_t h = u - lt * hp.heads;
+        const unsigned n = n0 + lt, b = fast_div(n, a.tdiv);
+        const int64_t t = n - b * static_cast<unsigned>(a.T);
+        src.x = static_cast<const T*>(hp.x) + (b * hp.xs[0] + t * hp.xs[1] + h * hp.xs[2]);
+        if constexpr (BWD) src.dy = static_cast<const T*>(hp.dy) + (b * hp.ds[0] + t * hp.ds[1] + h * hp.ds[2]);
+        dst.out = static_cast<T*>(hp.out) + (b * hp.os[0] + t * hp.os[1] + h * hp.os[2]);
+        dst.angles = lt * a.pstride;
+      }
+      sources[buf * a.rows + i] = src;
+      targets[buf * a.rows + i] = dst;
     }
     for (int i = tid; i < tokens * pairs; i += kHeadBlock) {
       const int lt = static_cast<int>(fast_div(static_cast<unsigned>(i), a.pdiv)), p = i - lt * pairs;
@@ -318,24 +356,17 @@ __global__ void __launch_bounds__(kHeadBlock, BWD ? 2 : 3) head_kernel(const Hea
 #pragma unroll
         for (int e = 0; e < V; ++e) xr[i][k].v[e] = dr[i][k].v[e] = Cvt<T>::from_f32(0.f);
   };
-  // Starts the loads of row `base + group` of a part's tile.
-  auto fetch = [&](int part, int buf, int base, int rows) {
-    const HeadPart& hp = a.part[part];
-    const int u = base + group;
-    if (u < rows) {
-      const unsigned lt = fast_div(static_cast<unsigned>(u), hp.div);
-      const int64_t h = u - static_cast<int>(lt) * hp.heads;
-      const int64_t* o = offsets + buf * buffer_offsets + part * OFFS * a.tile + lt;
-      const T* xp = static_cast<const T*>(hp.x) + o[a.tile] + h * hp.xs[2];
-      const T* dp = nullptr;
-      if constexpr (BWD) dp = static_cast<const T*>(hp.dy) + o[2 * a.tile] + h * hp.ds[2];
+  // Starts the loads of a row of a buffer.
+  auto fetch = [&](int at) {
+    const HeadSource src = sources[at];
+    if (src.x != nullptr) {
 #pragma unroll
       for (int i = 0; i < SPT; ++i)
 #pragma unroll
         for (int k = 0; k < 2; ++k)
           if (valid[i][k]) {
-            if constexpr (READ_X) xr[i][k] = load_stream<T, V>(xp, col[i][k]);
-            if constexpr (BWD) dr[i][k] = load_stream<T, V>(dp, col[i][k]);
+            if constexpr (READ_X) xr[i][k] = load_stream<T, V>(static_cast<const T*>(src.x), col[i][k]);
+            if constexpr (BWD) dr[i][k] = load_stream<T, V>(static_cast<const T*>(src.dy), col[i][k]);
           }
     } else if constexpr (BWD) {
       clear();   // a group without a row adds nothing to the parameter sums
@@ -346,20 +377,22 @@ __global__ void __launch_bounds__(kHeadBlock, BWD ? 2 : 3) head_kernel(const Hea
   const int64_t tile0 = blockIdx.x;
   make_tables(tile0, 0);
   __syncthreads();
-  fetch(0, 0, 0, tokens_of(tile0) * a.part[0].heads);
+  fetch(group);
   int buf = 0;
   for (int64_t tile = tile0; tile < a.tiles; tile += gridDim.x) {
     const bool more = tile + gridDim.x < a.tiles;
     const int next_buf = buf == 2 ? 0 : buf + 1;
     if (more) make_tables(tile + gridDim.x, next_buf);
     if (tile != tile0 || more) __syncthreads();
-    const int tokens = tokens_of(tile);
+    int64_t block;
+    int first;
+    place(tile, block, first);
     const float* tab = tables + buf * table_floats;
-    const int64_t* off = offsets + buf * buffer_offsets;
+    const int end = a.all_steps - first < a.steps ? a.all_steps - first : a.steps;
+    const int q_end = a.q_steps - first < end ? (a.q_steps > first ? a.q_steps - first : 0) : end;
 #pragma unroll 1
-    for (int part = 0; part < a.parts; ++part) {
-      const HeadPart& hp = a.part[part];
-      const int rows = tokens * hp.heads;
+    for (int part = q_end > 0 ? 0 : 1; part < a.parts; ++part) {
+      const int stop = part == 0 ? q_end : end;
       E g[SPT][2][NE], dg[SPT][2][NE], db[SPT][2][NE];
 #pragma unroll
       for (int i = 0; i < SPT; ++i)
@@ -374,17 +407,12 @@ __global__ void __launch_bounds__(kHeadBlock, BWD ? 2 : 3) head_kernel(const Hea
         for (int i = 0; i < SPT; ++i)
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            if (tile != tile0) {
-              head_sums_load<V>(mine, i * 2 + k, dg[i][k]);
-              if constexpr (NORM == 2) head_sums_load<V>(mine + 16 * kHeadBlock, i * 2 + k, db[i][k]);
-            } else {
-#pragma unroll
-              for (int e = 0; e < NE; ++e) dg[i][k][e] = db[i][k][e] = M::bcast(0.f);
-            }
+            head_sums_load<V>(mine, i * 2 + k, dg[i][k]);
+            if constexpr (NORM == 2) head_sums_load<V>(mine + 16 * kHeadBlock, i * 2 + k, db[i][k]);
           }
       }
 #pragma unroll 1
-      for (int base = 0; base < rows; base += groups) {
+      for (int step = part == 0 ? 0 : q_end; step < stop; ++step) {
         E x[SPT][2][NE], d[SPT][2][NE];
 #pragma unroll
         for (int i = 0; i < SPT; ++i)
@@ -393,23 +421,15 @@ __global__ void __launch_bounds__(kHeadBlock, BWD ? 2 : 3) head_kernel(const Hea
             if constexpr (READ_X) unpack<T, V>(xr[i][k], x[i][k]);
             if constexpr (BWD) unpack<T, V>(dr[i][k], d[i][k]);
           }
-        {  // the group's next row
-          int nb = base + groups, np = part;
-          bool nt = false;
-          if (nb >= rows) {
-            nb = 0;
-            if (++np == a.parts) np = 0, nt = true;
-          }
-          if (!nt) {
-            fetch(np, buf, nb, tokens * a.part[np].heads);
-          } else if (more) {
-            fetch(0, next_buf, 0, tokens_of(tile + gridDim.x) * a.part[0].heads);
-          }
+        // the group's next row, of this tile or the next
+        if (step + 1 < end) {
+          fetch(buf * a.rows + ((step + 1) << glog) + group);
+        } else if (more) {
+          fetch(next_buf * a.rows + group);
         }
-        const int u = base + group;
-        const bool on = u < rows;
-        const unsigned lt = on ? fast_div(static_cast<unsigned>(u), hp.div) : 0;
-        const float* tt = tab + lt * a.pstride;
+        const HeadTarget dst = targets[buf * a.rows + (step << glog) + group];
+        const bool on = dst.out != nullptr;
+        const float* tt = tab + dst.angles;
         if constexpr (BWD) head_rotate<V, IL, -1>(d, tt, lane, tph, rot);
         if constexpr (NORM == 2) {
           E acc = M::bcast(0.f);
@@ -488,8 +508,7 @@ __global__ void __launch_bounds__(kHeadBlock, BWD ? 2 : 3) head_kernel(const Hea
         }
         if constexpr (!BWD) head_rotate<V, IL, 1>(x, tt, lane, tph, rot);
         if (on) {
-          const int64_t h = u - static_cast<int>(lt) * hp.heads;
-          T* op = static_cast<T*>(hp.out) + off[part * OFFS * a.tile + lt] + h * hp.os[2];
+          T* op = static_cast<T*>(dst.out);
 #pragma unroll
           for (int i = 0; i < SPT; ++i)
 #pragma unroll

@@ -27,7 +27,8 @@ namespace nvn {
 namespace {
 
 constexpr bool kBwd = NVN_BWD != 0;
-constexpr int kTableBytes = 48 * 1024;   // most that a CTA's tables may take
+constexpr int kMaxRows = 256;            // of a tile (its addresses: 3 buffers of 32 bytes a row)
+constexpr int kTableBytes = 48 * 1024;   // most that a tile's angles may take
 
 inline int round4(int v) { return (v + 3) / 4 * 4; }
 
@@ -42,22 +43,31 @@ cudaError_t launch(HeadArgs& a, cudaStream_t s, bool dry_run, HeadPlan* plan) {
   if (a.tph > 32) return cudaErrorInvalidValue;
   a.pstride = a.tph * SPT * V * 2;
   a.hd4 = round4(a.hd);
-  // A tile holds eight rows for every group, less when that leaves SMs without a CTA.
-  const int heads = a.part[0].heads + (a.parts > 1 ? a.part[1].heads : 0);
+  // A tile is eight steps of the CTA, fewer when that leaves SMs without work: first fewer
+  // tokens, then a piece of one token's rows.
   const int groups = kHeadBlock / a.tph;
-  int64_t tile = heads > 0 ? (8 * groups + heads - 1) / heads : 1;
-  const int64_t spread = a.N / (static_cast<int64_t>(device_sm_count()) * 4);
-  if (tile > spread) tile = spread;
-  const int token_bytes = 3 * (a.pstride * 4 + 2 * (kBwd ? 3 : 2) * 8);
-  if (tile > kTableBytes / token_bytes) tile = kTableBytes / token_bytes;
+  const int hq = a.part[0].heads, hk = a.parts > 1 ? a.part[1].heads : 0;
+  const int most_steps = kMaxRows / groups < 8 ? kMaxRows / groups : 8;
+  const int64_t wanted = static_cast<int64_t>(device_sm_count()) * 4;   // tiles that keep every SM busy
+  int64_t tile = static_cast<int64_t>(most_steps) * groups / (hq + hk);
+  if (tile > a.N / wanted) tile = a.N / wanted;
+  if (tile > kTableBytes / (3 * 4 * a.pstride)) tile = kTableBytes / (3 * 4 * a.pstride);
   a.tile = static_cast<int>(tile < 1 ? 1 : tile);
-  a.tiles = (a.N + a.tile - 1) / a.tile;
+  const int64_t blocks = (a.N + a.tile - 1) / a.tile;
+  a.q_steps = static_cast<int>((static_cast<int64_t>(a.tile) * hq + groups - 1) / groups);
+  a.all_steps = a.q_steps + static_cast<int>((static_cast<int64_t>(a.tile) * hk + groups - 1) / groups);
+  a.steps = a.all_steps < most_steps + 2 ? a.all_steps : most_steps;
+  while (a.steps > 1 && blocks * ((a.all_steps + a.steps - 1) / a.steps) < wanted) --a.steps;
+  a.pieces = (a.all_steps + a.steps - 1) / a.steps;
+  a.tiles = blocks * a.pieces;
+  a.rows = a.steps * groups;
   const size_t fixed = static_cast<size_t>(2 * NV * a.hd4 + (kBwd ? 2 * NV * 16 * kHeadBlock : 0)) * 4;
-  const size_t smem = fixed + static_cast<size_t>(a.tile) * token_bytes;
+  const size_t smem = fixed + static_cast<size_t>(3) * (32 * a.rows + 4 * a.tile * a.pstride);
   static std::atomic<uint64_t> prepared{0};
   cudaError_t e = once_per_device(prepared, [&]() -> cudaError_t {
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                kTableBytes + (2 * NV * 512 + (kBwd ? 2 * NV * 16 * kHeadBlock : 0)) * 4);
+                                kTableBytes + 3 * 32 * (kMaxRows + 2 * kHeadBlock) +
+                                    (2 * NV * 512 + (kBwd ? 2 * NV * 16 * kHeadBlock : 0)) * 4);
   });
   if (e != cudaSuccess) return e;
   // persistent: tables and (backward) the parameter sums of a CTA serve all its tiles
@@ -88,7 +98,7 @@ cudaError_t launch(HeadArgs& a, cudaStream_t s, bool dry_run, HeadPlan* plan) {
   // dependent launches for short kernels only, as for the row kernels
   attr[0].val.programmaticStreamSerializationAllowed =
       use_dependent_launch() &&
-              a.N * heads * a.hd * static_cast<int64_t>(sizeof(T)) <= (int64_t(128) << 20)
+              a.N * (hq + hk) * a.hd * static_cast<int64_t>(sizeof(T)) <= (int64_t(128) << 20)
           ? 1
           : 0;
   cfg.attrs = attr;

@@ -334,7 +334,11 @@ struct HeadArgs {
   int pos64, axes, pairs;
   int64_t N, T, tiles;    // N = batch * tokens
   HeadDiv tdiv, pdiv;     // by T, by pairs
-  int hd, hd4, tph, tile, pstride;
+  int hd, hd4, tph, pstride;
+  int tile;               // tokens of a block
+  int q_steps, all_steps; // steps of a block: one row for every group of lanes each, queries first
+  int steps, pieces;      // steps of a tile, tiles of a block
+  int rows;               // rows of a tile
   float inv_hd, eps;
 };
 struct HeadPlan {
@@ -343,8 +347,7 @@ struct HeadPlan {
   size_t smem;
 };
 // `bwd`, `norm` (0 none, 1 root mean square, 2 mean and variance), `interleaved` select the
-// kernel; a.part / a.tile ... are filled in by the caller except tile, tiles, pstride, hd4, tph,
-// which the plan sets.  With dry_run nothing is launched.
+// kernel; the launcher sets the layout (hd4, tph, pstride, tile ... rows, tiles) itself.  With dry_run nothing is launched.
 #define NVN_DECLARE_HEADS(NAME)                                                                \
   cudaError_t NAME(int norm, bool interleaved, int v, HeadArgs& a, cudaStream_t s, bool dry_run, \
                    HeadPlan* plan);
