@@ -97,9 +97,11 @@ __device__ __forceinline__ float2 neg(float2 v) { return make_float2(-v.x, -v.y)
 __device__ __forceinline__ float neg(float v) { return -v; }
 
 // (a, b) -> (a cos - b sin, a sin + b cos), turned back for SIGN < 0.
+// `left` is the number of the slot's pairs that are rotated, for interleaved pairs whose rotated
+// range ends inside a vector (an infinity beside it must not meet a sine of zero).
 template <int V, bool IL, int SIGN, typename E, int NE>
 __device__ __forceinline__ void head_turn(E (&a)[NE], E (&b)[NE], const float (&c)[V],
-                                          const float (&sn)[V], bool rot_a, bool rot_b) {
+                                          const float (&sn)[V], bool rot_a, bool rot_b, int left) {
   using M = typename MathSel<V>::M;
   if constexpr (!IL || V == 1) {
     if (rot_a) {
@@ -119,28 +121,28 @@ __device__ __forceinline__ void head_turn(E (&a)[NE], E (&b)[NE], const float (&
       }
     }
   } else {
-    auto turn = [&](E& v, float cc, float ss) {
-      if (SIGN < 0) ss = -ss;
+    auto turn = [&](E& v, int e) {
+      const float cc = c[e], ss = SIGN < 0 ? -sn[e] : sn[e];
       const float u = fmaf(v.x, cc, -(v.y * ss));
-      v.y = fmaf(v.x, ss, v.y * cc);
-      v.x = u;
+      const float w = fmaf(v.x, ss, v.y * cc);
+      if (e < left) v = make_float2(u, w);
     };
     if (rot_a) {
 #pragma unroll
-      for (int e = 0; e < NE; ++e) turn(a[e], c[e], sn[e]);
+      for (int e = 0; e < NE; ++e) turn(a[e], e);
     }
     if (rot_b) {
 #pragma unroll
-      for (int e = 0; e < NE; ++e) turn(b[e], c[NE + e], sn[NE + e]);
+      for (int e = 0; e < NE; ++e) turn(b[e], NE + e);
     }
   }
 }
 
-template <int N>
+template <int FULL, int N>
 __device__ __forceinline__ void head_reduce(float (&v)[N], int tph) {
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) {
-    if (off < tph) {
+    if (off < (FULL != 0 ? FULL : tph)) {
 #pragma unroll
       for (int k = 0; k < N; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], off);
     }
@@ -200,15 +202,16 @@ __device__ __forceinline__ void head_sums_store(float* p, int j, const typename 
 }
 
 // Turns every slot of a row by its token's angles.
-template <int V, bool IL, int SIGN, int SPT, typename E, int NE>
+template <int V, bool IL, int SIGN, int FULL, int SPT, typename E, int NE>
 __device__ __forceinline__ void head_rotate(E (&v)[SPT][2][NE], const float* tab, int lane, int tph,
-                                            const bool (&rot)[SPT][2]) {
+                                            const bool (&rot)[SPT][2], int pairs) {
 #pragma unroll
   for (int i = 0; i < SPT; ++i) {
     float c[V], s[V];
     head_table_read<V>(tab, false, lane + i * tph, SPT * tph, c);
     head_table_read<V>(tab, true, lane + i * tph, SPT * tph, s);
-    head_turn<V, IL, SIGN>(v[i][0], v[i][1], c, s, rot[i][0], rot[i][1]);
+    head_turn<V, IL, SIGN>(v[i][0], v[i][1], c, s, rot[i][0], rot[i][1],
+                           FULL != 0 ? V : pairs - (lane + i * tph) * V);
   }
 }
 
@@ -224,7 +227,9 @@ struct alignas(16) HeadTarget {
 };
 
 // NORM: 0 none, 1 root mean square, 2 mean and variance.  IL: interleaved pairs.
-template <typename T, int V, int NORM, bool IL, bool BWD>
+// FULL: lanes per head when the head fills them exactly and every element is rotated (head_dim 64,
+// 128 or 256, no predicates and a fixed reduction); 0: any head.
+template <typename T, int V, int NORM, bool IL, bool BWD, int FULL>
 __global__ void __launch_bounds__(kHeadBlock, BWD ? 2 : 3) head_kernel(const HeadArgs a) {
   constexpr int SPT = HeadTraits<V>::SPT;
   using M = typename MathSel<V>::M;
@@ -245,7 +250,7 @@ __global__ void __launch_bounds__(kHeadBlock, BWD ? 2 : 3) head_kernel(const Hea
   const int table_floats = a.tile * a.pstride;
 
   const int tid = threadIdx.x;
-  const int tph = a.tph;
+  const int tph = FULL != 0 ? FULL : a.tph;
   const int lane = tid & (tph - 1);
   const int group = tid / tph;
   const int groups = kHeadBlock / tph;
@@ -256,20 +261,6 @@ __global__ void __launch_bounds__(kHeadBlock, BWD ? 2 : 3) head_kernel(const Hea
 
   griddep_launch_dependents();
   griddep_wait();
-  if constexpr (NV > 0) {
-    for (int i = tid; i < 2 * NV * a.hd4; i += kHeadBlock) {
-      const int which = i / a.hd4, col = i - which * a.hd4;
-      const float* src = NV == 1 ? a.param[2 * which] : a.param[which];
-      par[i] = src != nullptr && col < a.hd ? __ldg(src + col) : 0.f;
-    }
-  }
-  // slots behind the rotated pairs turn by nothing
-  for (int i = tid; i < 3 * a.tile * (nslots * V - pairs); i += kHeadBlock) {
-    const int row = i / (nslots * V - pairs), p = pairs + i - row * (nslots * V - pairs);
-    tables[row * a.pstride + head_table_at<V>(p, false, nslots)] = 1.f;
-    tables[row * a.pstride + head_table_at<V>(p, true, nslots)] = 0.f;
-  }
-
   // this thread's vectors
   int col[SPT][2];
   bool valid[SPT][2], rot[SPT][2];
@@ -279,13 +270,9 @@ __global__ void __launch_bounds__(kHeadBlock, BWD ? 2 : 3) head_kernel(const Hea
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       col[i][h] = head_col<V, IL>(s, h, pairs);
-      valid[i][h] = !IL && s * V < pairs ? true : 2 * s + h < vectors;
-      rot[i][h] = (!IL || V == 1) ? s * V < pairs : (2 * s + h) * V < 2 * pairs;
+      valid[i][h] = FULL != 0 || (!IL && s * V < pairs) || 2 * s + h < vectors;
+      rot[i][h] = FULL != 0 || ((!IL || V == 1) ? s * V < pairs : (2 * s + h) * V < 2 * pairs);
     }
-  }
-
-  if constexpr (BWD && NORM != 0) {
-    for (int i = tid; i < 2 * NV * 16 * kHeadBlock; i += kHeadBlock) sums[i] = 0.f;
   }
 
   // A tile's block of tokens and its first step (a step is one row for every group).
@@ -297,34 +284,42 @@ __global__ void __launch_bounds__(kHeadBlock, BWD ? 2 : 3) head_kernel(const Hea
       first = static_cast<int>(tile - block * a.pieces) * a.steps;
     }
   };
-  // The tables of a tile: angles, and where each row begins (nowhere for the rows that fill up a
-  // part's last step or lie behind the last token).
+  // Where row i of a tile begins; nowhere for the rows that fill up a part's last step or lie
+  // behind the last token.
+  auto row_at = [&](unsigned n0, int tokens, int first, int i, HeadSource& src, HeadTarget& dst) {
+    const int part = first + (i >> glog) >= a.q_steps ? 1 : 0;
+    const HeadPart& hp = a.part[part];
+    const int u = i + ((first - (part ? a.q_steps : 0)) << glog);
+    const int lt = static_cast<int>(fast_div(static_cast<unsigned>(u), hp.div));
+    src = {nullptr, nullptr};
+    dst = {nullptr, 0, 0};
+    if (lt < tokens) {
+      const int64_t h = u - lt * hp.heads;
+      const unsigned n = n0 + lt, b = fast_div(n, a.tdiv);
+      const int64_t t = n - b * static_cast<unsigned>(a.T);
+      src.x = static_cast<const T*>(hp.x) + (b * hp.xs[0] + t * hp.xs[1] + h * hp.xs[2]);
+      if constexpr (BWD) src.dy = static_cast<const T*>(hp.dy) + (b * hp.ds[0] + t * hp.ds[1] + h * hp.ds[2]);
+      dst.out = static_cast<T*>(hp.out) + (b * hp.os[0] + t * hp.os[1] + h * hp.os[2]);
+      dst.angles = lt * a.pstride;
+    }
+  };
+  auto tokens_of = [&](int64_t block) {
+    const int64_t left = a.N - block * a.tile;
+    return static_cast<int>(left < a.tile ? left : a.tile);
+  };
+  // The tables of a tile: angles, and where each row begins.
   auto make_tables = [&](int64_t tile, int buf) {
     int64_t block;
     int first;
     place(tile, block, first);
-    const int64_t left = a.N - block * a.tile;
-    const int tokens = static_cast<int>(left < a.tile ? left : a.tile);
+    const int tokens = tokens_of(block);
     const unsigned n0 = static_cast<unsigned>(block * a.tile);
     float* tab = tables + buf * table_floats;
     const int steps = a.all_steps - first < a.steps ? a.all_steps - first : a.steps;
     for (int i = tid; i < steps * groups; i += kHeadBlock) {
-      const int step = first + (i >> glog);
-      const int part = step >= a.q_steps ? 1 : 0;
-      const HeadPart& hp = a.part[part];
-      const int u = i + ((first - (part ? a.q_steps : 0)) << glog);
-      const int lt = static_cast<int>(fast_div(static_cast<unsigned>(u), hp.div));
-      HeadSource src = {nullptr, nullptr};
-      HeadTarget dst = {nullptr, 0, 0};
-      if (lt < tokens) {
-        const int64_t h = u - lt * hp.heads;
-        const unsigned n = n0 + lt, b = fast_div(n, a.tdiv);
-        const int64_t t = n - b * static_cast<unsigned>(a.T);
-        src.x = static_cast<const T*>(hp.x) + (b * hp.xs[0] + t * hp.xs[1] + h * hp.xs[2]);
-        if constexpr (BWD) src.dy = static_cast<const T*>(hp.dy) + (b * hp.ds[0] + t * hp.ds[1] + h * hp.ds[2]);
-        dst.out = static_cast<T*>(hp.out) + (b * hp.os[0] + t * hp.os[1] + h * hp.os[2]);
-        dst.angles = lt * a.pstride;
-      }
+      HeadSource src;
+      HeadTarget dst;
+      row_at(n0, tokens, first, i, src, dst);
       sources[buf * a.rows + i] = src;
       targets[buf * a.rows + i] = dst;
     }
@@ -357,8 +352,7 @@ __global__ void __launch_bounds__(kHeadBlock, BWD ? 2 : 3) head_kernel(const Hea
         for (int e = 0; e < V; ++e) xr[i][k].v[e] = dr[i][k].v[e] = Cvt<T>::from_f32(0.f);
   };
   // Starts the loads of a row of a buffer.
-  auto fetch = [&](int at) {
-    const HeadSource src = sources[at];
+  auto fetch = [&](const HeadSource src) {
     if (src.x != nullptr) {
 #pragma unroll
       for (int i = 0; i < SPT; ++i)
@@ -374,10 +368,37 @@ __global__ void __launch_bounds__(kHeadBlock, BWD ? 2 : 3) head_kernel(const Hea
   };
   clear();
 
+  auto fill_parameters = [&]() {
+    if constexpr (NV > 0) {
+      for (int i = tid; i < 2 * NV * a.hd4; i += kHeadBlock) {
+        const int which = i / a.hd4, col = i - which * a.hd4;
+        const float* src = NV == 1 ? a.param[2 * which] : a.param[which];
+        par[i] = src != nullptr && col < a.hd ? __ldg(src + col) : 0.f;
+      }
+    }
+    // slots behind the rotated pairs turn by nothing
+    for (int i = tid; i < 3 * a.tile * (nslots * V - pairs); i += kHeadBlock) {
+      const int row = i / (nslots * V - pairs), p = pairs + i - row * (nslots * V - pairs);
+      tables[row * a.pstride + head_table_at<V>(p, false, nslots)] = 1.f;
+      tables[row * a.pstride + head_table_at<V>(p, true, nslots)] = 0.f;
+    }
+    if constexpr (BWD && NORM != 0) {
+      for (int i = tid; i < 2 * NV * 16 * kHeadBlock; i += kHeadBlock) sums[i] = 0.f;
+    }
+  };
   const int64_t tile0 = blockIdx.x;
+  {  // the first row is on its way while the first tables are made
+    int64_t block;
+    int first;
+    place(tile0, block, first);
+    HeadSource src;
+    HeadTarget dst;
+    row_at(static_cast<unsigned>(block * a.tile), tokens_of(block), first, group, src, dst);
+    fetch(src);
+  }
   make_tables(tile0, 0);
+  fill_parameters();
   __syncthreads();
-  fetch(group);
   int buf = 0;
   for (int64_t tile = tile0; tile < a.tiles; tile += gridDim.x) {
     const bool more = tile + gridDim.x < a.tiles;
@@ -423,14 +444,14 @@ __global__ void __launch_bounds__(kHeadBlock, BWD ? 2 : 3) head_kernel(const Hea
           }
         // the group's next row, of this tile or the next
         if (step + 1 < end) {
-          fetch(buf * a.rows + ((step + 1) << glog) + group);
+          fetch(sources[buf * a.rows + ((step + 1) << glog) + group]);
         } else if (more) {
-          fetch(next_buf * a.rows + group);
+          fetch(sources[next_buf * a.rows + group]);
         }
         const HeadTarget dst = targets[buf * a.rows + (step << glog) + group];
         const bool on = dst.out != nullptr;
         const float* tt = tab + dst.angles;
-        if constexpr (BWD) head_rotate<V, IL, -1>(d, tt, lane, tph, rot);
+        if constexpr (BWD) head_rotate<V, IL, -1, FULL>(d, tt, lane, tph, rot, pairs);
         if constexpr (NORM == 2) {
           E acc = M::bcast(0.f);
 #pragma unroll
@@ -440,7 +461,7 @@ __global__ void __launch_bounds__(kHeadBlock, BWD ? 2 : 3) head_kernel(const Hea
 #pragma unroll
               for (int e = 0; e < NE; ++e) acc = M::add(acc, x[i][k][e]);
           float m[1] = {M::hsum(acc)};
-          head_reduce<1>(m, tph);
+          head_reduce<FULL>(m, tph);
           const E nm = M::bcast(-m[0] * a.inv_hd);
 #pragma unroll
           for (int i = 0; i < SPT; ++i)
@@ -471,7 +492,7 @@ __global__ void __launch_bounds__(kHeadBlock, BWD ? 2 : 3) head_kernel(const Hea
           float red[NR];
 #pragma unroll
           for (int k = 0; k < NR; ++k) red[k] = M::hsum(acc[k]) * a.inv_hd;  // shares of means: no overflow in the sum
-          head_reduce<NR>(red, tph);
+          head_reduce<FULL>(red, tph);
           // a group without a row must not put 0 * inf into the parameter sums
           const float inv = on ? rsqrtf(red[0] + a.eps) : 0.f;
           const E iv = M::bcast(inv);
@@ -506,7 +527,7 @@ __global__ void __launch_bounds__(kHeadBlock, BWD ? 2 : 3) head_kernel(const Hea
               }
           }
         }
-        if constexpr (!BWD) head_rotate<V, IL, 1>(x, tt, lane, tph, rot);
+        if constexpr (!BWD) head_rotate<V, IL, 1, FULL>(x, tt, lane, tph, rot, pairs);
         if (on) {
           T* op = static_cast<T*>(dst.out);
 #pragma unroll

@@ -76,7 +76,7 @@ int fill(const nvn_head_problem& p, const nvn_heads* const (&out)[2], const nvn_
   auto shrink = [&](const void* ptr, const int64_t(&s)[3]) {
     while (v > 1 && !fits(v, es, ptr, s)) v /= 2;
   };
-  while (v > 1 && (p.head_dim % v != 0 || (il ? 2 * p.pairs : p.pairs) % v != 0)) v /= 2;
+  while (v > 1 && (p.head_dim % v != 0 || (!il && p.pairs % v != 0))) v /= 2;
   for (int i = 0; i < a->parts; ++i) {
     HeadPart& h = a->part[i];
     h.heads = static_cast<int>(in[i]->heads);

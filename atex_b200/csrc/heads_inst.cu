@@ -32,9 +32,9 @@ constexpr int kTableBytes = 48 * 1024;   // most that a tile's angles may take
 
 inline int round4(int v) { return (v + 3) / 4 * 4; }
 
-template <int V, int NORM, bool IL>
-cudaError_t launch(HeadArgs& a, cudaStream_t s, bool dry_run, HeadPlan* plan) {
-  auto kernel = head_kernel<T, V, NORM, IL, kBwd>;
+template <int V, int NORM, bool IL, int FULL>
+cudaError_t launch_kernel(HeadArgs& a, cudaStream_t s, bool dry_run, HeadPlan* plan) {
+  auto kernel = head_kernel<T, V, NORM, IL, kBwd, FULL>;
   constexpr int SPT = HeadTraits<V>::SPT;
   constexpr int NV = NORM;
   const int slots = (a.hd + 2 * V - 1) / (2 * V);
@@ -43,21 +43,24 @@ cudaError_t launch(HeadArgs& a, cudaStream_t s, bool dry_run, HeadPlan* plan) {
   if (a.tph > 32) return cudaErrorInvalidValue;
   a.pstride = a.tph * SPT * V * 2;
   a.hd4 = round4(a.hd);
-  // A tile is eight steps of the CTA, fewer when that leaves SMs without work: first fewer
-  // tokens, then a piece of one token's rows.
+  // A tile is up to eight steps of the CTA.  Tokens are dealt out so that the CTAs that fit on the
+  // GPU at once take the same number of tiles; when there are fewer tokens than CTAs a tile is a
+  // piece of one token's rows.
   const int groups = kHeadBlock / a.tph;
   const int hq = a.part[0].heads, hk = a.parts > 1 ? a.part[1].heads : 0;
   const int most_steps = kMaxRows / groups < 8 ? kMaxRows / groups : 8;
-  const int64_t wanted = static_cast<int64_t>(device_sm_count()) * 4;   // tiles that keep every SM busy
+  const int64_t ctas = static_cast<int64_t>(device_sm_count()) * (kBwd ? 2 : 3);
   int64_t tile = static_cast<int64_t>(most_steps) * groups / (hq + hk);
-  if (tile > a.N / wanted) tile = a.N / wanted;
   if (tile > kTableBytes / (3 * 4 * a.pstride)) tile = kTableBytes / (3 * 4 * a.pstride);
-  a.tile = static_cast<int>(tile < 1 ? 1 : tile);
+  if (tile < 1) tile = 1;
+  const int64_t waves = (a.N + tile * ctas - 1) / (tile * ctas);
+  tile = (a.N + waves * ctas - 1) / (waves * ctas);
+  a.tile = static_cast<int>(tile);
   const int64_t blocks = (a.N + a.tile - 1) / a.tile;
   a.q_steps = static_cast<int>((static_cast<int64_t>(a.tile) * hq + groups - 1) / groups);
   a.all_steps = a.q_steps + static_cast<int>((static_cast<int64_t>(a.tile) * hk + groups - 1) / groups);
   a.steps = a.all_steps < most_steps + 2 ? a.all_steps : most_steps;
-  while (a.steps > 1 && blocks * ((a.all_steps + a.steps - 1) / a.steps) < wanted) --a.steps;
+  while (a.steps > 1 && blocks * ((a.all_steps + a.steps - 2) / (a.steps - 1)) <= ctas) --a.steps;
   a.pieces = (a.all_steps + a.steps - 1) / a.steps;
   a.tiles = blocks * a.pieces;
   a.rows = a.steps * groups;
@@ -105,6 +108,18 @@ cudaError_t launch(HeadArgs& a, cudaStream_t s, bool dry_run, HeadPlan* plan) {
   cfg.numAttrs = 1;
   count_launch();
   return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
+template <int V, int NORM, bool IL>
+cudaError_t launch(HeadArgs& a, cudaStream_t s, bool dry, HeadPlan* plan) {
+  if constexpr (V == VecTraits<T>::kFull) {
+    if (2 * a.pairs == a.hd) {
+      if (a.hd == 64) return launch_kernel<V, NORM, IL, 4>(a, s, dry, plan);
+      if (a.hd == 128) return launch_kernel<V, NORM, IL, 8>(a, s, dry, plan);
+      if (a.hd == 256) return launch_kernel<V, NORM, IL, 16>(a, s, dry, plan);
+    }
+  }
+  return launch_kernel<V, NORM, IL, 0>(a, s, dry, plan);
 }
 
 template <int V>
