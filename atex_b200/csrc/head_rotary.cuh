@@ -38,7 +38,11 @@
 
 namespace nvn {
 
-constexpr int kHeadBlock = 256;
+// Threads per CTA, and the CTAs per SM that the registers are limited for: with two rows at once
+// 5 (backward 3) small CTAs of up to 102 (168) registers; with one row 3 (2) of 80 (128).  Small
+// CTAs for one row were slower (f32 [3, 1025, 10+2, 80] gradient 17.5 -> 20.0 us).
+__host__ __device__ constexpr int head_block(int rows) { return rows > 1 ? 128 : 256; }
+__host__ __device__ constexpr int head_ctas(bool bwd, int rows) { return bwd ? (rows > 1 ? 3 : 2) : (rows > 1 ? 5 : 3); }
 
 // n / d for n < 2^31 by a multiplication: with 2^(s-1) < d <= 2^s and m = ceil(2^(31+s) / d),
 // m d - 2^(31+s) < d <= 2^s, so floor(n m / 2^(31+s)) is exact.
@@ -167,13 +171,13 @@ __device__ __forceinline__ void head_lanes(const float* p, typename MathSel<V>::
 }
 
 // The same, to shared memory of a thread's own: element e of vector j is word
-// ((j V + e) / CW) CW kHeadBlock + CW thread + e % CW, so that a warp's accesses are contiguous.
-template <int V>
+// ((j V + e) / CW) CW BLOCK + CW thread + e % CW, so that a warp's accesses are contiguous.
+template <int V, int BLOCK>
 __device__ __forceinline__ void head_sums_load(const float* p, int j, typename MathSel<V>::M::E (&out)[MathSel<V>::NE]) {
   constexpr int CW = HeadTraits<V>::CW;
 #pragma unroll
   for (int c = 0; c < V / CW; ++c) {
-    const float* q = p + (j * (V / CW) + c) * CW * kHeadBlock;
+    const float* q = p + (j * (V / CW) + c) * CW * BLOCK;
     if constexpr (CW == 4) {
       const float4 v = *reinterpret_cast<const float4*>(q);
       out[2 * c] = make_float2(v.x, v.y);
@@ -185,12 +189,12 @@ __device__ __forceinline__ void head_sums_load(const float* p, int j, typename M
     }
   }
 }
-template <int V>
+template <int V, int BLOCK>
 __device__ __forceinline__ void head_sums_store(float* p, int j, const typename MathSel<V>::M::E (&in)[MathSel<V>::NE]) {
   constexpr int CW = HeadTraits<V>::CW;
 #pragma unroll
   for (int c = 0; c < V / CW; ++c) {
-    float* q = p + (j * (V / CW) + c) * CW * kHeadBlock;
+    float* q = p + (j * (V / CW) + c) * CW * BLOCK;
     if constexpr (CW == 4) {
       *reinterpret_cast<float4*>(q) = make_float4(in[2 * c].x, in[2 * c].y, in[2 * c + 1].x, in[2 * c + 1].y);
     } else if constexpr (CW == 2) {
@@ -201,21 +205,23 @@ __device__ __forceinline__ void head_sums_store(float* p, int j, const typename 
   }
 }
 
-// Turns every slot of a row by its token's angles.
-template <int V, bool IL, int SIGN, int FULL, int SPT, typename E, int NE>
-__device__ __forceinline__ void head_rotate(E (&v)[SPT][2][NE], const float* tab, int lane, int tph,
+// Turns every slot of R rows of one token by its angles.
+template <int V, bool IL, int SIGN, int FULL, int R, int SPT, typename E, int NE>
+__device__ __forceinline__ void head_rotate(E (&v)[R][SPT][2][NE], const float* tab, int lane, int tph,
                                             const bool (&rot)[SPT][2], int pairs) {
 #pragma unroll
   for (int i = 0; i < SPT; ++i) {
     float c[V], s[V];
     head_table_read<V>(tab, false, lane + i * tph, SPT * tph, c);
     head_table_read<V>(tab, true, lane + i * tph, SPT * tph, s);
-    head_turn<V, IL, SIGN>(v[i][0], v[i][1], c, s, rot[i][0], rot[i][1],
-                           FULL != 0 ? V : pairs - (lane + i * tph) * V);
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      head_turn<V, IL, SIGN>(v[r][i][0], v[r][i][1], c, s, rot[i][0], rot[i][1],
+                             FULL != 0 ? V : pairs - (lane + i * tph) * V);
   }
 }
 
-// Where a row is read, and where it goes: null for a row that is none.
+// Where a row (the first of R) is read, and where it goes: null for one that is none.
 struct alignas(16) HeadSource {
   const void* x;
   const void* dy;
@@ -227,10 +233,13 @@ struct alignas(16) HeadTarget {
 };
 
 // NORM: 0 none, 1 root mean square, 2 mean and variance.  IL: interleaved pairs.
+// R: rows a group works on at once, neighbouring heads of one token: they share its angles and the
+// parameters, and their reductions overlap.
 // FULL: lanes per head when the head fills them exactly and every element is rotated (head_dim 64,
 // 128 or 256, no predicates and a fixed reduction); 0: any head.
-template <typename T, int V, int NORM, bool IL, bool BWD, int FULL>
-__global__ void __launch_bounds__(kHeadBlock, BWD ? 2 : 3) head_kernel(const HeadArgs a) {
+template <typename T, int V, int NORM, bool IL, bool BWD, int FULL, int R>
+__global__ void __launch_bounds__(head_block(R), head_ctas(BWD, R)) head_kernel(const HeadArgs a) {
+  constexpr int BLOCK = head_block(R);
   constexpr int SPT = HeadTraits<V>::SPT;
   using M = typename MathSel<V>::M;
   using E = typename M::E;
@@ -238,12 +247,12 @@ __global__ void __launch_bounds__(kHeadBlock, BWD ? 2 : 3) head_kernel(const Hea
   using P = Pack<T, V>;
   constexpr int NV = NORM;                         // parameter vectors per part
   constexpr bool READ_X = !BWD || NORM != 0;       // without a norm the gradient needs no x
-  // dynamic shared memory: gradient sums [2][NV][16][kHeadBlock] (backward), three buffers of row
+  // dynamic shared memory: gradient sums [2][NV][16][threads] (backward), three buffers of row
   // addresses [rows] (where x and dy are read; where the result goes, and the row's angles),
   // parameters [2][NV][hd4], three buffers of angles [tile][pstride]
   extern __shared__ __align__(16) float head_smem[];
   float* const sums = head_smem;
-  HeadSource* const sources = reinterpret_cast<HeadSource*>(sums + (BWD ? 2 * NV * 16 * kHeadBlock : 0));
+  HeadSource* const sources = reinterpret_cast<HeadSource*>(sums + (BWD ? 2 * NV * 16 * BLOCK : 0));
   HeadTarget* const targets = reinterpret_cast<HeadTarget*>(sources + 3 * a.rows);
   float* const par = reinterpret_cast<float*>(targets + 3 * a.rows);
   float* const tables = par + 2 * NV * a.hd4;
@@ -253,7 +262,7 @@ __global__ void __launch_bounds__(kHeadBlock, BWD ? 2 : 3) head_kernel(const Hea
   const int tph = FULL != 0 ? FULL : a.tph;
   const int lane = tid & (tph - 1);
   const int group = tid / tph;
-  const int groups = kHeadBlock / tph;
+  const int groups = BLOCK / tph;
   const int glog = 31 - __clz(groups);
   const int nslots = SPT * tph;
   const int pairs = a.pairs;
@@ -316,14 +325,14 @@ __global__ void __launch_bounds__(kHeadBlock, BWD ? 2 : 3) head_kernel(const Hea
     const unsigned n0 = static_cast<unsigned>(block * a.tile);
     float* tab = tables + buf * table_floats;
     const int steps = a.all_steps - first < a.steps ? a.all_steps - first : a.steps;
-    for (int i = tid; i < steps * groups; i += kHeadBlock) {
+    for (int i = tid; i < steps * groups; i += BLOCK) {
       HeadSource src;
       HeadTarget dst;
       row_at(n0, tokens, first, i, src, dst);
       sources[buf * a.rows + i] = src;
       targets[buf * a.rows + i] = dst;
     }
-    for (int i = tid; i < tokens * pairs; i += kHeadBlock) {
+    for (int i = tid; i < tokens * pairs; i += BLOCK) {
       const int lt = static_cast<int>(fast_div(static_cast<unsigned>(i), a.pdiv)), p = i - lt * pairs;
       const unsigned n = n0 + lt, b = fast_div(n, a.tdiv);
       const int64_t t = n - b * static_cast<unsigned>(a.T);
@@ -342,26 +351,33 @@ __global__ void __launch_bounds__(kHeadBlock, BWD ? 2 : 3) head_kernel(const Hea
     }
   };
 
-  P xr[SPT][2], dr[SPT][2];
+  P xr[R][SPT][2], dr[R][SPT][2];
   auto clear = [&]() {
 #pragma unroll
-    for (int i = 0; i < SPT; ++i)
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int e = 0; e < V; ++e) xr[i][k].v[e] = dr[i][k].v[e] = Cvt<T>::from_f32(0.f);
-  };
-  // Starts the loads of a row of a buffer.
-  auto fetch = [&](const HeadSource src) {
-    if (src.x != nullptr) {
+    for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int i = 0; i < SPT; ++i)
 #pragma unroll
         for (int k = 0; k < 2; ++k)
-          if (valid[i][k]) {
-            if constexpr (READ_X) xr[i][k] = load_stream<T, V>(static_cast<const T*>(src.x), col[i][k]);
-            if constexpr (BWD) dr[i][k] = load_stream<T, V>(static_cast<const T*>(src.dy), col[i][k]);
-          }
+#pragma unroll
+          for (int e = 0; e < V; ++e) xr[r][i][k].v[e] = dr[r][i][k].v[e] = Cvt<T>::from_f32(0.f);
+  };
+  // Starts the loads of a group's rows.
+  auto fetch = [&](const HeadSource src, int part) {
+    if (src.x != nullptr) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const T* xp = static_cast<const T*>(src.x) + (R > 1 ? r * a.part[part].x_row : 0);
+        const T* dp = static_cast<const T*>(src.dy) + (R > 1 ? r * a.part[part].d_row : 0);
+#pragma unroll
+        for (int i = 0; i < SPT; ++i)
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            if (valid[i][k]) {
+              if constexpr (READ_X) xr[r][i][k] = load_stream<T, V>(xp, col[i][k]);
+              if constexpr (BWD) dr[r][i][k] = load_stream<T, V>(dp, col[i][k]);
+            }
+      }
     } else if constexpr (BWD) {
       clear();   // a group without a row adds nothing to the parameter sums
     }
@@ -370,20 +386,20 @@ __global__ void __launch_bounds__(kHeadBlock, BWD ? 2 : 3) head_kernel(const Hea
 
   auto fill_parameters = [&]() {
     if constexpr (NV > 0) {
-      for (int i = tid; i < 2 * NV * a.hd4; i += kHeadBlock) {
+      for (int i = tid; i < 2 * NV * a.hd4; i += BLOCK) {
         const int which = i / a.hd4, col = i - which * a.hd4;
         const float* src = NV == 1 ? a.param[2 * which] : a.param[which];
         par[i] = src != nullptr && col < a.hd ? __ldg(src + col) : 0.f;
       }
     }
     // slots behind the rotated pairs turn by nothing
-    for (int i = tid; i < 3 * a.tile * (nslots * V - pairs); i += kHeadBlock) {
+    for (int i = tid; i < 3 * a.tile * (nslots * V - pairs); i += BLOCK) {
       const int row = i / (nslots * V - pairs), p = pairs + i - row * (nslots * V - pairs);
       tables[row * a.pstride + head_table_at<V>(p, false, nslots)] = 1.f;
       tables[row * a.pstride + head_table_at<V>(p, true, nslots)] = 0.f;
     }
     if constexpr (BWD && NORM != 0) {
-      for (int i = tid; i < 2 * NV * 16 * kHeadBlock; i += kHeadBlock) sums[i] = 0.f;
+      for (int i = tid; i < 2 * NV * 16 * BLOCK; i += BLOCK) sums[i] = 0.f;
     }
   };
   const int64_t tile0 = blockIdx.x;
@@ -394,7 +410,7 @@ __global__ void __launch_bounds__(kHeadBlock, BWD ? 2 : 3) head_kernel(const Hea
     HeadSource src;
     HeadTarget dst;
     row_at(static_cast<unsigned>(block * a.tile), tokens_of(block), first, group, src, dst);
-    fetch(src);
+    fetch(src, first < a.q_steps ? 0 : 1);
   }
   make_tables(tile0, 0);
   fill_parameters();
@@ -410,10 +426,18 @@ __global__ void __launch_bounds__(kHeadBlock, BWD ? 2 : 3) head_kernel(const Hea
     place(tile, block, first);
     const float* tab = tables + buf * table_floats;
     const int end = a.all_steps - first < a.steps ? a.all_steps - first : a.steps;
+    int next_part = 0;
+    if (more) {
+      int64_t next_block;
+      int next_first;
+      place(tile + gridDim.x, next_block, next_first);
+      next_part = next_first < a.q_steps ? 0 : 1;
+    }
     const int q_end = a.q_steps - first < end ? (a.q_steps > first ? a.q_steps - first : 0) : end;
 #pragma unroll 1
     for (int part = q_end > 0 ? 0 : 1; part < a.parts; ++part) {
       const int stop = part == 0 ? q_end : end;
+      const HeadPart& hp = a.part[part];
       E g[SPT][2][NE], dg[SPT][2][NE], db[SPT][2][NE];
 #pragma unroll
       for (int i = 0; i < SPT; ++i)
@@ -422,125 +446,146 @@ __global__ void __launch_bounds__(kHeadBlock, BWD ? 2 : 3) head_kernel(const Hea
           if constexpr (NORM != 0)
             head_lanes<V>(par + part * NV * a.hd4 + (valid[i][k] ? col[i][k] : 0), g[i][k]);
         }
-      float* const mine = sums + part * NV * 16 * kHeadBlock + tid * HeadTraits<V>::CW;
+      float* const mine = sums + part * NV * 16 * BLOCK + tid * HeadTraits<V>::CW;
       if constexpr (BWD && NORM != 0) {
 #pragma unroll
         for (int i = 0; i < SPT; ++i)
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            head_sums_load<V>(mine, i * 2 + k, dg[i][k]);
-            if constexpr (NORM == 2) head_sums_load<V>(mine + 16 * kHeadBlock, i * 2 + k, db[i][k]);
+            head_sums_load<V, BLOCK>(mine, i * 2 + k, dg[i][k]);
+            if constexpr (NORM == 2) head_sums_load<V, BLOCK>(mine + 16 * BLOCK, i * 2 + k, db[i][k]);
           }
       }
 #pragma unroll 1
       for (int step = part == 0 ? 0 : q_end; step < stop; ++step) {
-        E x[SPT][2][NE], d[SPT][2][NE];
+        E x[R][SPT][2][NE], d[R][SPT][2][NE];
 #pragma unroll
-        for (int i = 0; i < SPT; ++i)
+        for (int r = 0; r < R; ++r)
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            if constexpr (READ_X) unpack<T, V>(xr[i][k], x[i][k]);
-            if constexpr (BWD) unpack<T, V>(dr[i][k], d[i][k]);
-          }
-        // the group's next row, of this tile or the next
+          for (int i = 0; i < SPT; ++i)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              if constexpr (READ_X) unpack<T, V>(xr[r][i][k], x[r][i][k]);
+              if constexpr (BWD) unpack<T, V>(dr[r][i][k], d[r][i][k]);
+            }
+        // the group's next rows, of this tile or the next
         if (step + 1 < end) {
-          fetch(sources[buf * a.rows + ((step + 1) << glog) + group]);
+          fetch(sources[buf * a.rows + ((step + 1) << glog) + group], step + 1 < q_end ? 0 : 1);
         } else if (more) {
-          fetch(sources[next_buf * a.rows + group]);
+          fetch(sources[next_buf * a.rows + group], next_part);
         }
         const HeadTarget dst = targets[buf * a.rows + (step << glog) + group];
         const bool on = dst.out != nullptr;
         const float* tt = tab + dst.angles;
-        if constexpr (BWD) head_rotate<V, IL, -1, FULL>(d, tt, lane, tph, rot, pairs);
+        if constexpr (BWD) head_rotate<V, IL, -1, FULL, R>(d, tt, lane, tph, rot, pairs);
         if constexpr (NORM == 2) {
-          E acc = M::bcast(0.f);
+          float m[R];
 #pragma unroll
-          for (int i = 0; i < SPT; ++i)
+          for (int r = 0; r < R; ++r) {
+            E acc = M::bcast(0.f);
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
+            for (int i = 0; i < SPT; ++i)
 #pragma unroll
-              for (int e = 0; e < NE; ++e) acc = M::add(acc, x[i][k][e]);
-          float m[1] = {M::hsum(acc)};
+              for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int e = 0; e < NE; ++e) acc = M::add(acc, x[r][i][k][e]);
+            m[r] = M::hsum(acc);
+          }
           head_reduce<FULL>(m, tph);
-          const E nm = M::bcast(-m[0] * a.inv_hd);
 #pragma unroll
-          for (int i = 0; i < SPT; ++i)
+          for (int r = 0; r < R; ++r) {
+            const E nm = M::bcast(-m[r] * a.inv_hd);
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
+            for (int i = 0; i < SPT; ++i)
 #pragma unroll
-              for (int e = 0; e < NE; ++e) x[i][k][e] = valid[i][k] ? M::add(x[i][k][e], nm) : M::bcast(0.f);
+              for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int e = 0; e < NE; ++e)
+                  x[r][i][k][e] = valid[i][k] ? M::add(x[r][i][k][e], nm) : M::bcast(0.f);
+          }
         }
         if constexpr (NORM != 0) {
           // sum of squares; backward: sum gy c and, for mean and variance, sum gy beside it
           constexpr int NR = BWD ? NORM + 1 : 1;
-          E acc[NR];
+          float red[NR * R];
 #pragma unroll
-          for (int k = 0; k < NR; ++k) acc[k] = M::bcast(0.f);
+          for (int r = 0; r < R; ++r) {
+            E acc[NR];
 #pragma unroll
-          for (int i = 0; i < SPT; ++i)
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-#pragma unroll
-              for (int e = 0; e < NE; ++e) {
-                acc[0] = M::fma(x[i][k][e], x[i][k][e], acc[0]);
-                if constexpr (BWD) {
-                  const E gy = M::mul(d[i][k][e], g[i][k][e]);
-                  acc[1] = M::fma(gy, x[i][k][e], acc[1]);
-                  if constexpr (NORM == 2) acc[NORM] = M::add(acc[NORM], gy);
-                }
-              }
-          float red[NR];
-#pragma unroll
-          for (int k = 0; k < NR; ++k) red[k] = M::hsum(acc[k]) * a.inv_hd;  // shares of means: no overflow in the sum
-          head_reduce<FULL>(red, tph);
-          // a group without a row must not put 0 * inf into the parameter sums
-          const float inv = on ? rsqrtf(red[0] + a.eps) : 0.f;
-          const E iv = M::bcast(inv);
-          if constexpr (BWD) {
-            const E nm1 = M::bcast(-red[1] * inv);
-            const E nm0 = M::bcast(NORM == 2 ? -red[NORM] : 0.f);
+            for (int k = 0; k < NR; ++k) acc[k] = M::bcast(0.f);
 #pragma unroll
             for (int i = 0; i < SPT; ++i)
 #pragma unroll
               for (int k = 0; k < 2; ++k)
 #pragma unroll
                 for (int e = 0; e < NE; ++e) {
-                  const E xh = M::mul(x[i][k][e], iv);
-                  dg[i][k][e] = M::fma(d[i][k][e], xh, dg[i][k][e]);
-                  if constexpr (NORM == 2) db[i][k][e] = M::add(db[i][k][e], d[i][k][e]);
-                  const E gy = NORM == 2 ? M::fma(d[i][k][e], g[i][k][e], nm0) : M::mul(d[i][k][e], g[i][k][e]);
-                  d[i][k][e] = M::mul(M::fma(nm1, xh, gy), iv);
+                  acc[0] = M::fma(x[r][i][k][e], x[r][i][k][e], acc[0]);
+                  if constexpr (BWD) {
+                    const E gy = M::mul(d[r][i][k][e], g[i][k][e]);
+                    acc[1] = M::fma(gy, x[r][i][k][e], acc[1]);
+                    if constexpr (NORM == 2) acc[NORM] = M::add(acc[NORM], gy);
+                  }
                 }
-          } else {
+#pragma unroll
+            for (int k = 0; k < NR; ++k)
+              red[r * NR + k] = M::hsum(acc[k]) * a.inv_hd;  // shares of means: no overflow in the sum
+          }
+          head_reduce<FULL>(red, tph);
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            // a group without a row must not put 0 * inf into the parameter sums
+            const float inv = on ? rsqrtf(red[r * NR] + a.eps) : 0.f;
+            const E iv = M::bcast(inv);
+            if constexpr (BWD) {
+              const E nm1 = M::bcast(-red[r * NR + 1] * inv);
+              const E nm0 = M::bcast(NORM == 2 ? -red[r * NR + NORM] : 0.f);
+#pragma unroll
+              for (int i = 0; i < SPT; ++i)
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                  for (int e = 0; e < NE; ++e) {
+                    E& de = d[r][i][k][e];
+                    const E xh = M::mul(x[r][i][k][e], iv);
+                    dg[i][k][e] = M::fma(de, xh, dg[i][k][e]);
+                    if constexpr (NORM == 2) db[i][k][e] = M::add(db[i][k][e], de);
+                    const E gy = NORM == 2 ? M::fma(de, g[i][k][e], nm0) : M::mul(de, g[i][k][e]);
+                    de = M::mul(M::fma(nm1, xh, gy), iv);
+                  }
+            } else {
+#pragma unroll
+              for (int i = 0; i < SPT; ++i)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                  E be[NE];   // the offsets stay in shared memory: registers are short here
+                  if constexpr (NORM == 2)
+                    head_lanes<V>(par + (part * NV + 1) * a.hd4 + (valid[i][k] ? col[i][k] : 0), be);
+#pragma unroll
+                  for (int e = 0; e < NE; ++e) {
+                    const E xh = M::mul(x[r][i][k][e], iv);
+                    x[r][i][k][e] = NORM == 2 ? M::fma(xh, g[i][k][e], be[e]) : M::mul(xh, g[i][k][e]);
+                  }
+                }
+            }
+          }
+        }
+        if constexpr (!BWD) head_rotate<V, IL, 1, FULL, R>(x, tt, lane, tph, rot, pairs);
+        if (on) {
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            T* op = static_cast<T*>(dst.out) + (R > 1 ? r * hp.o_row : 0);
 #pragma unroll
             for (int i = 0; i < SPT; ++i)
 #pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                E be[NE];   // the offsets stay in shared memory: registers are short here
-                if constexpr (NORM == 2)
-                  head_lanes<V>(par + (part * NV + 1) * a.hd4 + (valid[i][k] ? col[i][k] : 0), be);
-#pragma unroll
-                for (int e = 0; e < NE; ++e) {
-                  const E xh = M::mul(x[i][k][e], iv);
-                  x[i][k][e] = NORM == 2 ? M::fma(xh, g[i][k][e], be[e]) : M::mul(xh, g[i][k][e]);
+              for (int k = 0; k < 2; ++k)
+                if (valid[i][k]) {
+                  if constexpr (BWD) {
+                    store_stream<T, V>(op, col[i][k], repack<T, V>(d[r][i][k]));
+                  } else {
+                    store_stream<T, V>(op, col[i][k], repack<T, V>(x[r][i][k]));
+                  }
                 }
-              }
           }
-        }
-        if constexpr (!BWD) head_rotate<V, IL, 1, FULL>(x, tt, lane, tph, rot, pairs);
-        if (on) {
-          T* op = static_cast<T*>(dst.out);
-#pragma unroll
-          for (int i = 0; i < SPT; ++i)
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-              if (valid[i][k]) {
-                if constexpr (BWD) {
-                  store_stream<T, V>(op, col[i][k], repack<T, V>(d[i][k]));
-                } else {
-                  store_stream<T, V>(op, col[i][k], repack<T, V>(x[i][k]));
-                }
-              }
         }
       }
       if constexpr (BWD && NORM != 0) {
@@ -548,8 +593,8 @@ __global__ void __launch_bounds__(kHeadBlock, BWD ? 2 : 3) head_kernel(const Hea
         for (int i = 0; i < SPT; ++i)
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            head_sums_store<V>(mine, i * 2 + k, dg[i][k]);
-            if constexpr (NORM == 2) head_sums_store<V>(mine + 16 * kHeadBlock, i * 2 + k, db[i][k]);
+            head_sums_store<V, BLOCK>(mine, i * 2 + k, dg[i][k]);
+            if constexpr (NORM == 2) head_sums_store<V, BLOCK>(mine + 16 * BLOCK, i * 2 + k, db[i][k]);
           }
       }
     }
@@ -561,7 +606,7 @@ __global__ void __launch_bounds__(kHeadBlock, BWD ? 2 : 3) head_kernel(const Hea
     __syncthreads();
     float* w = a.ws + static_cast<int64_t>(blockIdx.x) * a.parts * NV * a.hd;
     constexpr int CW = HeadTraits<V>::CW;
-    for (int o = tid; o < a.parts * NV * 16 * tph; o += kHeadBlock) {
+    for (int o = tid; o < a.parts * NV * 16 * tph; o += BLOCK) {
       const int vec = o / (16 * tph), rest = o - vec * 16 * tph;
       const int el = rest / tph, ln = rest - el * tph;
       const int s = ln + el / (2 * V) * tph, half = el / V % 2;
@@ -569,7 +614,7 @@ __global__ void __launch_bounds__(kHeadBlock, BWD ? 2 : 3) head_kernel(const Hea
       if (!in) continue;
       float t = 0.f;
       for (int gr = 0; gr < groups; ++gr)
-        t += sums[(vec * 16 + el / CW * CW) * kHeadBlock + (gr * tph + ln) * CW + el % CW];
+        t += sums[(vec * 16 + el / CW * CW) * BLOCK + (gr * tph + ln) * CW + el % CW];
       w[vec * a.hd + head_col<V, IL>(s, half, pairs) + el % V] = t;
     }
   }

@@ -10,14 +10,6 @@ namespace {
 constexpr int64_t kMaxHeadDim = 512;    // 32 lanes of 16 elements
 constexpr int64_t kMaxHeads = 65535;
 
-HeadDiv divider(int64_t d) {
-  if (d <= 1) return {0, -1};
-  int s = 1;
-  while ((int64_t(1) << s) < d) ++s;
-  const uint64_t m = ((uint64_t(1) << (31 + s)) + static_cast<uint64_t>(d) - 1) / static_cast<uint64_t>(d);
-  return {static_cast<unsigned>(m), s - 1};
-}
-
 typedef cudaError_t (*HeadsFn)(int, bool, int, HeadArgs&, cudaStream_t, bool, HeadPlan*);
 HeadsFn heads_fn(int dtype, bool bwd) {
   if (dtype == NVN_F32) return bwd ? heads_f32_bwd : heads_f32_fwd;
@@ -80,7 +72,6 @@ int fill(const nvn_head_problem& p, const nvn_heads* const (&out)[2], const nvn_
   for (int i = 0; i < a->parts; ++i) {
     HeadPart& h = a->part[i];
     h.heads = static_cast<int>(in[i]->heads);
-    h.div = divider(h.heads);
     h.x = in[i]->data;
     strides(p, *in[i], h.xs);
     shrink(h.x, h.xs);
@@ -110,8 +101,8 @@ int fill(const nvn_head_problem& p, const nvn_heads* const (&out)[2], const nvn_
   a->pairs = static_cast<int>(p.pairs);
   a->N = p.batch * p.tokens;
   a->T = p.tokens;
-  a->tdiv = divider(p.tokens);
-  a->pdiv = divider(p.pairs);
+  a->tdiv = head_divider(p.tokens);
+  a->pdiv = head_divider(p.pairs);
   a->hd = static_cast<int>(p.head_dim);
   a->inv_hd = 1.0f / static_cast<float>(p.head_dim);
   a->eps = p.epsilon;

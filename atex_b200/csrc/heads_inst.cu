@@ -32,9 +32,10 @@ constexpr int kTableBytes = 48 * 1024;   // most that a tile's angles may take
 
 inline int round4(int v) { return (v + 3) / 4 * 4; }
 
-template <int V, int NORM, bool IL, int FULL>
-cudaError_t launch_kernel(HeadArgs& a, cudaStream_t s, bool dry_run, HeadPlan* plan) {
-  auto kernel = head_kernel<T, V, NORM, IL, kBwd, FULL>;
+template <int V, int NORM, bool IL, int FULL, int R>
+cudaError_t launch_kernel(HeadArgs a, cudaStream_t s, bool dry_run, HeadPlan* plan) {
+  auto kernel = head_kernel<T, V, NORM, IL, kBwd, FULL, R>;
+  constexpr int BLOCK = head_block(R);
   constexpr int SPT = HeadTraits<V>::SPT;
   constexpr int NV = NORM;
   const int slots = (a.hd + 2 * V - 1) / (2 * V);
@@ -46,10 +47,21 @@ cudaError_t launch_kernel(HeadArgs& a, cudaStream_t s, bool dry_run, HeadPlan* p
   // A tile is up to eight steps of the CTA.  Tokens are dealt out so that the CTAs that fit on the
   // GPU at once take the same number of tiles; when there are fewer tokens than CTAs a tile is a
   // piece of one token's rows.
-  const int groups = kHeadBlock / a.tph;
+  const int groups = BLOCK / a.tph;
+  for (int i = 0; i < a.parts; ++i) {   // R heads are one row of work
+    HeadPart& h = a.part[i];
+    h.heads /= R;
+    h.div = head_divider(h.heads);
+    h.x_row = h.xs[2];
+    h.d_row = h.ds[2];
+    h.o_row = h.os[2];
+    h.xs[2] *= R;
+    h.ds[2] *= R;
+    h.os[2] *= R;
+  }
   const int hq = a.part[0].heads, hk = a.parts > 1 ? a.part[1].heads : 0;
-  const int most_steps = kMaxRows / groups < 8 ? kMaxRows / groups : 8;
-  const int64_t ctas = static_cast<int64_t>(device_sm_count()) * (kBwd ? 2 : 3);
+  const int most_steps = kMaxRows / R / groups < 8 ? kMaxRows / R / groups : 8;
+  const int64_t ctas = static_cast<int64_t>(device_sm_count()) * head_ctas(kBwd, R);
   int64_t tile = static_cast<int64_t>(most_steps) * groups / (hq + hk);
   if (tile > kTableBytes / (3 * 4 * a.pstride)) tile = kTableBytes / (3 * 4 * a.pstride);
   if (tile < 1) tile = 1;
@@ -64,13 +76,13 @@ cudaError_t launch_kernel(HeadArgs& a, cudaStream_t s, bool dry_run, HeadPlan* p
   a.pieces = (a.all_steps + a.steps - 1) / a.steps;
   a.tiles = blocks * a.pieces;
   a.rows = a.steps * groups;
-  const size_t fixed = static_cast<size_t>(2 * NV * a.hd4 + (kBwd ? 2 * NV * 16 * kHeadBlock : 0)) * 4;
+  const size_t fixed = static_cast<size_t>(2 * NV * a.hd4 + (kBwd ? 2 * NV * 16 * BLOCK : 0)) * 4;
   const size_t smem = fixed + static_cast<size_t>(3) * (32 * a.rows + 4 * a.tile * a.pstride);
   static std::atomic<uint64_t> prepared{0};
   cudaError_t e = once_per_device(prepared, [&]() -> cudaError_t {
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                kTableBytes + 3 * 32 * (kMaxRows + 2 * kHeadBlock) +
-                                    (2 * NV * 512 + (kBwd ? 2 * NV * 16 * kHeadBlock : 0)) * 4);
+                                kTableBytes + 3 * 32 * (kMaxRows + 2 * BLOCK) +
+                                    (2 * NV * 512 + (kBwd ? 2 * NV * 16 * BLOCK : 0)) * 4);
   });
   if (e != cudaSuccess) return e;
   // persistent: tables and (backward) the parameter sums of a CTA serve all its tiles
@@ -80,7 +92,7 @@ cudaError_t launch_kernel(HeadArgs& a, cudaStream_t s, bool dry_run, HeadPlan* p
   if (c != 0 && static_cast<size_t>(c >> 20) == smem) {
     per_sm = static_cast<int>(c & 0xfffff);
   } else {
-    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kHeadBlock, smem);
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, BLOCK, smem);
     if (e != cudaSuccess) return e;
     if (per_sm < 1) per_sm = 1;
     cached.store((static_cast<int64_t>(smem) << 20) | per_sm, std::memory_order_relaxed);
@@ -93,7 +105,7 @@ cudaError_t launch_kernel(HeadArgs& a, cudaStream_t s, bool dry_run, HeadPlan* p
   if (dry_run) return cudaSuccess;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
-  cfg.blockDim = dim3(kHeadBlock, 1, 1);
+  cfg.blockDim = dim3(BLOCK, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -101,7 +113,7 @@ cudaError_t launch_kernel(HeadArgs& a, cudaStream_t s, bool dry_run, HeadPlan* p
   // dependent launches for short kernels only, as for the row kernels
   attr[0].val.programmaticStreamSerializationAllowed =
       use_dependent_launch() &&
-              a.N * (hq + hk) * a.hd * static_cast<int64_t>(sizeof(T)) <= (int64_t(128) << 20)
+              a.N * (hq + hk) * R * a.hd * static_cast<int64_t>(sizeof(T)) <= (int64_t(128) << 20)
           ? 1
           : 0;
   cfg.attrs = attr;
@@ -110,16 +122,30 @@ cudaError_t launch_kernel(HeadArgs& a, cudaStream_t s, bool dry_run, HeadPlan* p
   return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
+template <int V, int NORM, bool IL, int R>
+cudaError_t launch_full(HeadArgs& a, cudaStream_t s, bool dry, HeadPlan* plan) {
+  if (a.hd == 64) return launch_kernel<V, NORM, IL, 4, R>(a, s, dry, plan);
+  if (a.hd == 128) return launch_kernel<V, NORM, IL, 8, R>(a, s, dry, plan);
+  return launch_kernel<V, NORM, IL, 16, R>(a, s, dry, plan);
+}
+
 template <int V, int NORM, bool IL>
 cudaError_t launch(HeadArgs& a, cudaStream_t s, bool dry, HeadPlan* plan) {
   if constexpr (V == VecTraits<T>::kFull) {
-    if (2 * a.pairs == a.hd) {
-      if (a.hd == 64) return launch_kernel<V, NORM, IL, 4>(a, s, dry, plan);
-      if (a.hd == 128) return launch_kernel<V, NORM, IL, 8>(a, s, dry, plan);
-      if (a.hd == 256) return launch_kernel<V, NORM, IL, 16>(a, s, dry, plan);
+    if (2 * a.pairs == a.hd && (a.hd == 64 || a.hd == 128 || a.hd == 256)) {
+      // two heads at once in 16 bits, when they pair up and there is work for every CTA; fp32 rows
+      // are twice as long and would not fit in the registers
+      if constexpr (sizeof(T) == 2) {
+        const int hq = a.part[0].heads, hk = a.parts > 1 ? a.part[1].heads : 0;
+        const int groups = head_block(1) / (a.hd / 16);
+        if (hq % 2 == 0 && hk % 2 == 0 &&
+            a.N * (hq + hk) >= static_cast<int64_t>(device_sm_count()) * head_ctas(kBwd, 1) * groups)
+          return launch_full<V, NORM, IL, 2>(a, s, dry, plan);
+      }
+      return launch_full<V, NORM, IL, 1>(a, s, dry, plan);
     }
   }
-  return launch_kernel<V, NORM, IL, 0>(a, s, dry, plan);
+  return launch_kernel<V, NORM, IL, 0, 1>(a, s, dry, plan);
 }
 
 template <int V>

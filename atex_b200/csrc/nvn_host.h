@@ -319,9 +319,17 @@ struct HeadPart {  // the queries or the keys
   const void* dy;
   void* out;
   int64_t xs[3], ds[3], os[3];
-  int heads;
+  int64_t x_row, d_row, o_row;  // between the heads of a group of rows
+  int heads;       // groups of rows per token
   HeadDiv div;     // by heads
 };
+inline HeadDiv head_divider(int64_t d) {
+  if (d <= 1) return {0, -1};
+  int s = 1;
+  while ((int64_t(1) << s) < d) ++s;
+  const uint64_t m = ((uint64_t(1) << (31 + s)) + static_cast<uint64_t>(d) - 1) / static_cast<uint64_t>(d);
+  return {static_cast<unsigned>(m), s - 1};
+}
 struct HeadArgs {
   HeadPart part[2];
   int parts;
