@@ -23,9 +23,9 @@ from typing import Iterable
 import torch
 
 from . import _lib
-from .nv_norm_ops import (InvalidArgumentError, LayerNormalization, _axis_list, _check, _device_guard,
-                          _dtype_code, _grad_outputs, _like_output, _ln_dims, _on_device, _param,
-                          _require, _stream, _ws_bytes, fused_layer_norm_grad_op,
+from .nv_norm_ops import (InvalidArgumentError, LayerNormalization, _axis_list, _check, _dtype_code,
+                          _grad_outputs, _like_output, _ln_dims, _on_device, _param, _remember,
+                          _require, _ws_bytes, fused_layer_norm_grad_op,
                           fused_layer_norm_residual_op)
 
 __all__ = [
@@ -35,22 +35,41 @@ __all__ = [
 ]
 
 
-def _scratch(device: torch.device, nbytes: int) -> torch.Tensor:
-    """Workspace of one call.  From the caching allocator on the current stream, so that calls on
+def _on_stream(index: int, fn, *args) -> int:
+    """fn(*args, stream) with device `index` current, on torch's current stream of that device."""
+    if torch._C._cuda_getDevice() == index:
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+
+
+def _scratch(like: torch.Tensor, nbytes: int) -> torch.Tensor:
+    """Workspace of one call, `like` a float32 tensor of the device.  nbytes is a multiple of 256.  From the caching allocator on the current stream, so that calls on
     different streams and captured graphs never share one, and a captured graph owns its own."""
-    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return like.new_empty(nbytes // 4)
+
+
+# The checks of x and scale depend on their shapes and types alone; a small decoding step spends
+# more time in them than the GPU in the kernel, so what has passed is remembered (bounded).
+_rows_cache = {}
 
 
 def _rows(x, scale, axis):
     """Checks x and scale against each other: (dtype code, N, D)."""
+    try:
+        key = (x.shape, x.dtype, scale.shape, scale.dtype, axis)
+        return _rows_cache[key]
+    except (KeyError, AttributeError, TypeError):
+        pass
     _require(isinstance(x, torch.Tensor) and x.dim() > 0, "input must be at least 1-dimensional",
              x if isinstance(x, torch.Tensor) else "")
     code = _dtype_code(x, "x")
     _param(scale, "scale")
-    N, D = _ln_dims(x, _axis_list(axis))
+    axis = tuple(_axis_list(axis))
+    N, D = _ln_dims(x, axis)
     _require(scale.numel() == D, "scale must have the same number of elements as the features "
              "of x, got ", scale.numel(), " and ", D)
-    return code, N, D
+    return _remember(_rows_cache, (x.shape, x.dtype, scale.shape, scale.dtype, axis), (code, N, D))
 
 
 def _like_x(t, x, name):
@@ -67,6 +86,12 @@ def _saved(t, name, N):
 
 def _together(*named):
     """Contiguous CUDA tensors, all on one device."""
+    device = named[0][0].device
+    for t, _ in named:
+        if not (t.is_cuda and t.is_contiguous() and t.device == device):
+            break
+    else:
+        return [t for t, _ in named]
     out = _on_device(*named)
     for t, (_, name) in zip(out, named):
         if t.device != out[0].device:
@@ -74,12 +99,21 @@ def _together(*named):
     return out
 
 
-def _one_output(like_numel, device, out, name):
+def _one_output(like_numel, scale, out, name):
     if out is None:
-        return torch.empty(like_numel, dtype=torch.float32, device=device)
+        return scale.new_empty(like_numel)
+    device = scale.device
     if out.dtype != torch.float32 or out.numel() != like_numel or not out.is_contiguous() or out.device != device:
         raise ValueError(f"{name} must be a contiguous float32 tensor of {like_numel} elements on {device}")
     return out
+
+
+def _on_device_bytes(index: int, fn_name: str, *args) -> int:
+    """A workspace size, asked for with device `index` current (and remembered)."""
+    if torch._C._cuda_getDevice() == index:
+        return _ws_bytes(fn_name, *args)
+    with torch.cuda.device(index):
+        return _ws_bytes(fn_name, *args)
 
 
 # ---------------------------------------------------------------------------
@@ -94,10 +128,9 @@ def fused_rms_norm_op(x, scale, axis: Iterable[int] = (-1,), epsilon: float = 0.
     code, N, D = _rows(x, scale, axis)
     x, scale = _together((x, "x"), (scale, "scale"))
     y = _like_output(x, out, "out")
-    inv = _one_output(N, x.device, out_stats, "out_stats")
-    with _device_guard(x.device):
-        st = _lib.load().nvn_rms_fwd(code, x.data_ptr(), scale.data_ptr(), N, D, float(epsilon), y.data_ptr(),
-                                     inv.data_ptr(), _stream(x.device))
+    inv = _one_output(N, scale, out_stats, "out_stats")
+    st = _on_stream(x.get_device(), _lib.load().nvn_rms_fwd, code, x.data_ptr(), scale.data_ptr(), N, D,
+                    float(epsilon), y.data_ptr(), inv.data_ptr())
     _check(st, "nvn_rms_fwd")
     return y, inv
 
@@ -117,11 +150,9 @@ def fused_rms_norm_residual_op(x, residual, scale, axis: Iterable[int] = (-1,), 
     s = _like_output(x, out_sum, "out_sum")
     if N * D and y.data_ptr() == s.data_ptr():
         raise ValueError("out and out_sum must be different tensors")
-    inv = _one_output(N, x.device, out_stats, "out_stats")
-    with _device_guard(x.device):
-        st = _lib.load().nvn_rms_fwd_residual(code, x.data_ptr(), residual.data_ptr(), scale.data_ptr(), N, D,
-                                              float(epsilon), s.data_ptr(), y.data_ptr(), inv.data_ptr(),
-                                              _stream(x.device))
+    inv = _one_output(N, scale, out_stats, "out_stats")
+    st = _on_stream(x.get_device(), _lib.load().nvn_rms_fwd_residual, code, x.data_ptr(), residual.data_ptr(),
+                    scale.data_ptr(), N, D, float(epsilon), s.data_ptr(), y.data_ptr(), inv.data_ptr())
     _check(st, "nvn_rms_fwd_residual")
     return y, s, inv
 
@@ -137,13 +168,13 @@ def _rms_grad(dy, dsum, x, scale, inv, axis, out_grads, out):
         x, dy, dsum, scale, inv = _together((x, "x"), (dy, "y_backprop"), (dsum, "sum_backprop"), (scale, "scale"),
                                             (inv, "reserve_space_1"))
     dx = _like_output(x, out, "out")
-    dscale = torch.empty_like(scale) if out_grads is None else _one_output(D, x.device, out_grads, "out_grads")
-    with _device_guard(x.device):
-        nbytes = _ws_bytes("nvn_rms_bwd_workspace_bytes", code, N, D)
-        ws = _scratch(x.device, nbytes)
-        st = _lib.load().nvn_rms_bwd(code, dy.data_ptr(), 0 if dsum is None else dsum.data_ptr(), x.data_ptr(),
-                                     scale.data_ptr(), inv.data_ptr(), N, D, dx.data_ptr(), dscale.data_ptr(),
-                                     ws.data_ptr(), nbytes, _stream(x.device))
+    dscale = torch.empty_like(scale) if out_grads is None else _one_output(D, scale, out_grads, "out_grads")
+    index = x.get_device()
+    nbytes = _on_device_bytes(index, "nvn_rms_bwd_workspace_bytes", code, N, D)
+    ws = _scratch(scale, nbytes)
+    st = _on_stream(index, _lib.load().nvn_rms_bwd, code, dy.data_ptr(), 0 if dsum is None else dsum.data_ptr(),
+                    x.data_ptr(), scale.data_ptr(), inv.data_ptr(), N, D, dx.data_ptr(), dscale.data_ptr(),
+                    ws.data_ptr(), nbytes)
     _check(st, "nvn_rms_bwd")
     return dx, dscale
 
@@ -187,13 +218,12 @@ def fused_layer_norm_residual_grad_op(y_backprop, sum_backprop, s, scale, reserv
                                               (reserve_space_2, "reserve_space_2"))
     dx = _like_output(x, out, "out")
     dscale, doffset = _grad_outputs(scale, out_grads)
-    with _device_guard(x.device):
-        nbytes = _ws_bytes("nvn_ln_bwd_residual_workspace_bytes", code, N, D)
-        ws = _scratch(x.device, nbytes)
-        st = _lib.load().nvn_ln_bwd_residual(code, dy.data_ptr(), dsum.data_ptr(), x.data_ptr(), scale.data_ptr(),
-                                             mean.data_ptr(), inv.data_ptr(), N, D, dx.data_ptr(),
-                                             dscale.data_ptr(), doffset.data_ptr(), ws.data_ptr(), nbytes,
-                                             _stream(x.device))
+    index = x.get_device()
+    nbytes = _on_device_bytes(index, "nvn_ln_bwd_residual_workspace_bytes", code, N, D)
+    ws = _scratch(scale, nbytes)
+    st = _on_stream(index, _lib.load().nvn_ln_bwd_residual, code, dy.data_ptr(), dsum.data_ptr(), x.data_ptr(),
+                    scale.data_ptr(), mean.data_ptr(), inv.data_ptr(), N, D, dx.data_ptr(), dscale.data_ptr(),
+                    doffset.data_ptr(), ws.data_ptr(), nbytes)
     _check(st, "nvn_ln_bwd_residual")
     return dx, dscale, doffset
 

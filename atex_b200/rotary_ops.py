@@ -26,8 +26,8 @@ from typing import Sequence, Tuple
 import torch
 
 from . import _lib
-from .nv_norm_ops import (InvalidArgumentError, _check, _device_guard, _dtype_code, _param, _require,
-                          _stream)
+from .nv_norm_ops import InvalidArgumentError, _check, _dtype_code, _param, _remember, _require
+from .rms_norm_ops import _on_stream, _scratch
 
 __all__ = ["fused_head_norm_rotary_op", "fused_head_norm_rotary_grad_op", "head_norm_rotary",
            "rotary_frequencies", "HeadNormRotary"]
@@ -80,12 +80,6 @@ def _rows_contiguous(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _pack(t):
-    """(data, heads, stride of batch, token, head) of a view."""
-    s = t.stride()
-    return (t.data_ptr(), t.shape[-2], s[0] if len(s) == 4 else 0, s[-3], s[-2])
-
-
 def _checked_out(t, like, name):
     if (not isinstance(t, torch.Tensor) or t.shape != like.shape or t.dtype != like.dtype
             or t.device != like.device):
@@ -100,13 +94,13 @@ def _checked_out(t, like, name):
     return t
 
 
-class _Problem:
-    """The checked arguments both directions share."""
+class _Form:
+    """What the two directions need of a call's shapes, types, strides and options, once checked."""
 
     def __init__(self, q, k, positions, inv_freq, pair_axis, scales, offsets, norm, interleaved, epsilon,
                  want_offsets):
         B, T, H, D = _heads(q, "q")
-        self.code = _dtype_code(q, "q")
+        code = _dtype_code(q, "q")
         if k is not None:
             kb, kt, kh, kd = _heads(k, "k")
             _require(k.dim() == q.dim() and (kb, kt, kd) == (B, T, D),
@@ -117,9 +111,8 @@ class _Problem:
         _require(H > 0 and D > 0, "q must have at least one head and one element in it, got ", q)
         if norm not in _NORMS:
             raise InvalidArgumentError(f"norm must be 'rms', 'layer' or 'none', got {norm!r}")
-        self.norm, self.vectors = _NORMS[norm]
-        self.parts = 1 if k is None else 2
-        self.shape, self.head_dim = (B, T, H, D), D
+        norm_code, self.vectors = _NORMS[norm]
+        self.parts, self.head_dim = 1 if k is None else 2, D
         tensors = [(q, "q")] + ([(k, "k")] if k is not None else [])
         for what, given, wanted in (("scale", scales, norm != "none"),
                                     ("offset", offsets, norm == "layer" and want_offsets)):
@@ -133,8 +126,8 @@ class _Problem:
                 _require(t.numel() == D, name, " must have the same number of elements as a head, got ", t.numel(),
                          " and ", D)
                 tensors.append((t, name))
-        self.pairs = self.axes = 0
-        pos = (0, 0, 0, 0, 0)
+        pairs = axes = 0
+        pos = (0, 0, 0)
         if positions is not None:
             if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.int64):
                 raise TypeError("positions must be an int32 or int64 tensor")
@@ -148,38 +141,98 @@ class _Problem:
             _require(inv_freq.dim() == 1 and inv_freq.shape == pair_axis.shape,
                      "inv_freq and pair_axis must be 1-dimensional and of one length, got ", inv_freq, " and ",
                      pair_axis)
-            self.pairs, self.axes = inv_freq.numel(), positions.shape[0]
-            _require(2 * self.pairs <= D, "inv_freq has ", self.pairs, " pairs, a head has only ", D, " elements")
+            pairs, axes = inv_freq.numel(), positions.shape[0]
+            _require(2 * pairs <= D, "inv_freq has ", pairs, " pairs, a head has only ", D, " elements")
             tensors += [(positions, "positions"), (inv_freq, "inv_freq"), (pair_axis, "pair_axis")]
+            s = positions.stride()
+            pos = (s[0], s[1] if len(s) == 3 else 0, s[-1])
         else:
             _require(inv_freq is None and pair_axis is None, "inv_freq and pair_axis need positions")
         for t, name in tensors:
             _on_cuda(t, name, q.device)
-        self.q, self.k = _rows_contiguous(q), None if k is None else _rows_contiguous(k)
-        self.params = [None if t is None else t.contiguous() for t in (scales[0], offsets[0], scales[1], offsets[1])]
-        self.freq = None if positions is None else inv_freq.contiguous()
-        self.axis = None if positions is None else pair_axis.contiguous()
-        self.positions = positions
-        if positions is not None:
-            s = positions.stride()
-            pos = (positions.data_ptr(), s[0], s[1] if len(s) == 3 else 0, s[-1],
-                   4 if positions.dtype == torch.int32 else 8)
-        self.packed = _PROBLEM.pack(
-            self.code, self.norm, int(bool(interleaved)), float(epsilon), B, T, D, self.pairs, self.axes, pos[4],
-            pos[0], pos[1], pos[2], pos[3], 0 if self.freq is None else self.freq.data_ptr(),
-            0 if self.axis is None else self.axis.data_ptr(), *_pack(self.q),
-            *((0, 0, 0, 0, 0) if self.k is None else _pack(self.k)),
-            *[0 if t is None else t.data_ptr() for t in self.params])
+        # views that the kernels cannot read are copied at every call
+        self.copies = not all(t is None or t.is_contiguous() for t in (*scales, *offsets, inv_freq, pair_axis))
+        self.copies = self.copies or any(t is not None and _rows_contiguous(t) is not t for t in (q, k))
+        self.empty = B * T == 0
+        position_bytes = 8 if positions is None or positions.dtype == torch.int64 else 4
+        self.head = (code, norm_code, int(bool(interleaved)), float(epsilon), B, T, D, pairs, axes, position_bytes)
+        self.pos = pos
+        self.q = _layout(q)
+        self.k = (0, 0, 0, 0) if k is None else _layout(k)
+        self.workspace = None
 
-    def outputs(self, out):
-        if out is None:
-            return (torch.empty(self.q.shape, dtype=self.q.dtype, device=self.q.device),
-                    None if self.k is None else torch.empty(self.k.shape, dtype=self.q.dtype, device=self.q.device))
-        q_out, k_out = out
-        _checked_out(q_out, self.q, "out[0]")
-        if self.k is not None:
-            _checked_out(k_out, self.k, "out[1]")
-        return q_out, k_out
+    def workspace_bytes(self, index):
+        """Of the gradient, at the widest accesses the strides allow (addresses may narrow them)."""
+        if self.workspace is None:
+            if self.vectors == 0 or self.empty:
+                self.workspace = 0
+            else:
+                somewhere = 1 << 20   # an address of full alignment; a size query reads nothing
+                packed = _PROBLEM.pack(*self.head, somewhere, *self.pos, somewhere, somewhere, somewhere, *self.q,
+                                       somewhere if self.parts > 1 else 0, *self.k, *([somewhere] * 4))
+                with torch.cuda.device(index):
+                    self.workspace = int(_lib.load().nvn_head_norm_rotary_bwd_workspace_bytes(packed))
+        return self.workspace
+
+
+def _layout(t):
+    """(heads, strides of batch, token and head) of a view."""
+    s = t.stride()
+    return (t.shape[-2], s[0] if len(s) == 4 else 0, s[-3], s[-2])
+
+
+def _key(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+
+
+# A call's checks depend on shapes, types, strides, devices and options alone, and a decoding step
+# spends more time in them than the GPU in the kernel: what has passed is remembered (bounded).
+_forms = {}
+
+
+def _problem(q, k, positions, inv_freq, pair_axis, scales, offsets, norm, interleaved, epsilon, want_offsets):
+    """The checked form of a call, its nvn_head_problem, and q and k as the kernels can read them."""
+    try:
+        key = (_key(q), _key(k), _key(positions), _key(inv_freq), _key(pair_axis), _key(scales[0]), _key(scales[1]),
+               _key(offsets[0]), _key(offsets[1]), norm, interleaved, epsilon, want_offsets)
+        form = _forms.get(key)
+    except (AttributeError, TypeError):
+        form = key = None
+    if form is None:
+        form = _Form(q, k, positions, inv_freq, pair_axis, scales, offsets, norm, interleaved, epsilon, want_offsets)
+        if key is not None:
+            _remember(_forms, key, form)
+    params = (scales[0], offsets[0], scales[1], offsets[1])
+    layouts = form.q, form.k
+    if form.copies:
+        params = [None if t is None else t.contiguous() for t in params]
+        inv_freq = None if inv_freq is None else inv_freq.contiguous()
+        pair_axis = None if pair_axis is None else pair_axis.contiguous()
+        q, k = _rows_contiguous(q), None if k is None else _rows_contiguous(k)
+        layouts = _layout(q), form.k if k is None else _layout(k)
+    packed = _PROBLEM.pack(*form.head, _ptr(positions), *form.pos, _ptr(inv_freq), _ptr(pair_axis), q.data_ptr(),
+                           *layouts[0], _ptr(k), *layouts[1], *[_ptr(t) for t in params])
+    # the copies must outlive the launch that reads them
+    return form, packed, q, k, (params, inv_freq, pair_axis)
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _pack(t):
+    """nvn_heads of a view."""
+    return None if t is None else _HEADS.pack(t.data_ptr(), *_layout(t))
+
+
+def _outputs(q, k, out):
+    if out is None:
+        return q.new_empty(q.shape), None if k is None else k.new_empty(k.shape)
+    q_out, k_out = out
+    _checked_out(q_out, q, "out[0]")
+    if k is not None:
+        _checked_out(k_out, k, "out[1]")
+    return q_out, k_out
 
 
 def fused_head_norm_rotary_op(q, k, positions, inv_freq=None, pair_axis=None, scale_q=None, scale_k=None,
@@ -193,16 +246,12 @@ def fused_head_norm_rotary_op(q, k, positions, inv_freq=None, pair_axis=None, sc
     one of positions' is not rotated).  Scales and offsets are float32 of head_dim elements.
     ``out`` = (q_out, k_out) supplies the outputs as views of any layout; they may be q and k
     themselves."""
-    p = _Problem(q, k, positions, inv_freq, pair_axis, (scale_q, scale_k), (offset_q, offset_k), norm,
-                 interleaved, epsilon, True)
-    q_out, k_out = p.outputs(out)
-    if q.numel() == 0:
+    form, packed, q, k, alive = _problem(q, k, positions, inv_freq, pair_axis, (scale_q, scale_k),
+                                         (offset_q, offset_k), norm, interleaved, epsilon, True)
+    q_out, k_out = _outputs(q, k, out)
+    if form.empty:
         return q_out, k_out
-    device = p.q.device
-    with _device_guard(device):
-        st = _lib.load().nvn_head_norm_rotary_fwd(p.packed, _HEADS.pack(*_pack(q_out)),
-                                                  None if k is None else _HEADS.pack(*_pack(k_out)),
-                                                  _stream(device))
+    st = _on_stream(q.get_device(), _lib.load().nvn_head_norm_rotary_fwd, packed, _pack(q_out), _pack(k_out))
     _check(st, "nvn_head_norm_rotary_fwd")
     return q_out, k_out
 
@@ -214,38 +263,36 @@ def fused_head_norm_rotary_grad_op(q_backprop, k_backprop, q, k, positions, inv_
     doffset_q, doffset_k), with None for what the form does not have.  The statistics are formed
     again from q and k.  ``out`` = (dq, dk) supplies those as views of any layout, for example the
     slices of a packed projection's gradient; they may be q_backprop and k_backprop themselves."""
-    p = _Problem(q, k, positions, inv_freq, pair_axis, (scale_q, scale_k), (None, None), norm, interleaved,
-                 epsilon, False)
+    form, packed, q, k, alive = _problem(q, k, positions, inv_freq, pair_axis, (scale_q, scale_k), (None, None), norm,
+                                         interleaved, epsilon, False)
     _require((k is None) == (k_backprop is None), "k_backprop belongs to k")
-    grads = []
-    for g, x, name in ((q_backprop, q, "q_backprop"), (k_backprop, k, "k_backprop")):
-        if x is None:
-            grads.append(None)
-            continue
-        if not isinstance(g, torch.Tensor) or g.shape != x.shape or g.dtype != x.dtype:
-            raise InvalidArgumentError(f"{name} must have the shape and dtype of its input")
-        _on_cuda(g, name, x.device)
-        grads.append(_rows_contiguous(g))
-    dq, dk = p.outputs(out)
-    device, D = p.q.device, p.head_dim
-    if p.vectors:
-        fresh = torch.zeros if q.numel() == 0 else torch.empty
-        dparams = fresh((p.parts, p.vectors, D), dtype=torch.float32, device=device)
-    if q.numel():
-        lib = _lib.load()
-        with _device_guard(device):
-            nbytes = lib.nvn_head_norm_rotary_bwd_workspace_bytes(p.packed) if p.vectors else 0
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-            st = lib.nvn_head_norm_rotary_bwd(
-                p.packed, _HEADS.pack(*_pack(grads[0])), None if k is None else _HEADS.pack(*_pack(grads[1])),
-                _HEADS.pack(*_pack(dq)), None if k is None else _HEADS.pack(*_pack(dk)),
-                dparams.data_ptr() if p.vectors else None, None if ws is None else ws.data_ptr(), nbytes,
-                _stream(device))
+    grads = [None, None]
+    for i, (g, x, name) in enumerate(((q_backprop, q, "q_backprop"), (k_backprop, k, "k_backprop"))):
+        if x is not None:
+            if not isinstance(g, torch.Tensor) or g.shape != x.shape or g.dtype != x.dtype:
+                raise InvalidArgumentError(f"{name} must have the shape and dtype of its input")
+            _on_cuda(g, name, x.device)
+            grads[i] = _rows_contiguous(g)
+    dq, dk = _outputs(q, k, out)
+    dparams = ws = None
+    if form.vectors:
+        dparams = scale_q.new_empty((form.parts * form.vectors, form.head_dim))
+        if form.empty:
+            dparams.zero_()
+    if not form.empty:
+        index = q.get_device()
+        nbytes = form.workspace_bytes(index)
+        if nbytes:
+            ws = _scratch(scale_q, nbytes)
+        st = _on_stream(index, _lib.load().nvn_head_norm_rotary_bwd, packed, _pack(grads[0]), _pack(grads[1]),
+                        _pack(dq), _pack(dk), _ptr(dparams), _ptr(ws), nbytes)
         _check(st, "nvn_head_norm_rotary_bwd")
-    if not p.vectors:
+    if dparams is None:
         return dq, dk, None, None, None, None
-    sums = [[dparams[i, j] if i < p.parts and j < p.vectors else None for i in range(2)] for j in range(2)]
-    return dq, dk, sums[0][0], sums[0][1], sums[1][0], sums[1][1]
+    sums = dparams.unbind() + (None,) * 4   # scale (and offset) of q, then of k
+    if form.vectors == 1:
+        return dq, dk, sums[0], sums[1], None, None
+    return dq, dk, sums[0], sums[2], sums[1], sums[3]
 
 
 class _head_norm_rotary_grad(torch.autograd.Function):
