@@ -12,28 +12,24 @@ namespace nvn {
 namespace {
 
 struct Shape {
-  int tpr, vpt, cs, pf;
+  int capacity, pf, forms;
 };
-#define X(I, TPR, VPT, CS, RB, PR, MINB, PF) {TPR, VPT, CS, PF},
-const Shape kFwdShapes[] = {NVN_ROW_SHAPES_LIGHT(X)};
-const Shape kBwdShapes[] = {NVN_ROW_SHAPES_HEAVY(X)};
-const Shape kNarrowShapes[] = {NVN_ROW_SHAPES_SCALAR(X)};
+#define X(I, TPR, VPT, RB, MINB, PF, FORMS) {TPR * VPT, PF, FORMS},
+const Shape kFwdShapes[] = {NVN_RMS_FWD_SHAPES(X)};
+const Shape kBwdShapes[] = {NVN_RMS_BWD_SHAPES(X)};
+const Shape kNarrowShapes[] = {NVN_RMS_NARROW_SHAPES(X)};
 #undef X
 
-// Bytes per tensor from which a held ring (the row batch stays in shared memory between the
-// two passes of the gradient) beats register prefetch; the value found for LayerNorm.
-constexpr int64_t kHeldMinBytes = 64ll << 20;
-
-// Smallest one-CTA shape that holds `nvec` accesses, or -1; held rings only for large tensors
+// Smallest shape of the form that holds `nvec` accesses, or -1; held rings only for large tensors
 // unless nothing else fits.
-int pick(const Shape* table, int n, int64_t nvec, int64_t tensor_bytes) {
+int pick(const Shape* table, int n, int form, int64_t nvec, int64_t tensor_bytes) {
   int best = -1;
   for (int pass = 0; pass < 2 && best < 0; ++pass)
     for (int i = 0; i < n; ++i) {
-      const int64_t cap = static_cast<int64_t>(table[i].tpr) * table[i].vpt;
-      if (table[i].cs != 1 || cap < nvec) continue;
-      if (pass == 0 && table[i].pf >= 10 && tensor_bytes < kHeldMinBytes) continue;
-      if (best < 0 || cap < static_cast<int64_t>(table[best].tpr) * table[best].vpt) best = i;
+      const Shape& t = table[i];
+      if ((t.forms >> form & 1) == 0 || t.capacity < nvec) continue;
+      if (pass == 0 && t.pf >= 10 && tensor_bytes < kRmsHeldMinBytes) continue;
+      if (best < 0 || t.capacity < table[best].capacity) best = i;
     }
   return best;
 }
@@ -60,7 +56,7 @@ int plan(int form, int dtype, bool bwd, int64_t N, int64_t D, size_t align, size
   const int64_t tensor_bytes = N * D * static_cast<int64_t>(dtype_size(dtype));
   const Shape* table = !full ? kNarrowShapes : (bwd ? kBwdShapes : kFwdShapes);
   const size_t count = !full ? sizeof(kNarrowShapes) : (bwd ? sizeof(kBwdShapes) : sizeof(kFwdShapes));
-  p->shape = pick(table, static_cast<int>(count / sizeof(Shape)), D / p->epv, tensor_bytes);
+  p->shape = pick(table, static_cast<int>(count / sizeof(Shape)), form, D / p->epv, tensor_bytes);
   if (!bwd) return NVN_OK;
   if (p->shape >= 0) {
     RowsResArgs a = {};

@@ -6,9 +6,8 @@
 //   backward   xh = x inv, gy = dy g:  dx = inv (gy - xh mean(gy xh)) [+ dsum],  dg = sum dy xh
 //              and the LayerNorm gradient with dsum (its plain form is in rows_inst.cu)
 //
-// A row belongs to one CTA (no cluster shapes): 4096 vectors forward, 2048 backward; wider
-// rows take rows_generic.cu.  The tables are the LayerNorm kernels' own shapes without the
-// cluster entries.
+// A row belongs to one CTA: up to 4096 vectors forward, 2048 backward; wider rows take
+// rows_generic.cu.
 #include "rows_kernels.cuh"
 
 #if NVN_T == 0
@@ -115,28 +114,28 @@ cudaError_t launch_exact(const RowsResArgs& a, cudaStream_t stream, bool dry_run
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<const Args&>(a));
 }
 
-template <int EPV, int TPR, int VPT, int CS, int RB, bool PR, int MINB, int PF, int FORM>
+template <int EPV, int TPR, int VPT, int RB, int MINB, int PF, int FORMS, int FORM>
 cudaError_t launch_one(const RowsResArgs& a, cudaStream_t s, bool dry, RowsPlan* plan) {
-  if constexpr (CS > 1) {
-    return cudaErrorInvalidValue;  // cluster shapes are not part of this family
+  if constexpr ((FORMS >> FORM & 1) == 0) {
+    return cudaErrorInvalidValue;  // another form's entry
   } else {
     return a.D == static_cast<int64_t>(TPR) * VPT * EPV
-               ? launch_exact<EPV, TPR, VPT, RB, PR, MINB, PF, true, FORM>(a, s, dry, plan)
-               : launch_exact<EPV, TPR, VPT, RB, PR, MINB, PF, false, FORM>(a, s, dry, plan);
+               ? launch_exact<EPV, TPR, VPT, RB, true, MINB, PF, true, FORM>(a, s, dry, plan)
+               : launch_exact<EPV, TPR, VPT, RB, true, MINB, PF, false, FORM>(a, s, dry, plan);
   }
 }
 
 template <int EPV, int FORM>
 cudaError_t launch_form(int shape, const RowsResArgs& a, cudaStream_t s, bool dry, RowsPlan* plan) {
-#define X(I, TPR, VPT, CS, RB, PR, MINB, PF) \
-  case I:                                    \
-    return launch_one<EPV, TPR, VPT, CS, RB, PR != 0, MINB, PF, FORM>(a, s, dry, plan);
+#define X(I, TPR, VPT, RB, MINB, PF, FORMS) \
+  case I:                                   \
+    return launch_one<EPV, TPR, VPT, RB, MINB, PF, FORMS, FORM>(a, s, dry, plan);
   if constexpr (EPV != VecTraits<T>::kFull) {
-    switch (shape) { NVN_ROW_SHAPES_SCALAR(X) }
+    switch (shape) { NVN_RMS_NARROW_SHAPES(X) }
   } else if constexpr (kBwd) {
-    switch (shape) { NVN_ROW_SHAPES_HEAVY(X) }
+    switch (shape) { NVN_RMS_BWD_SHAPES(X) }
   } else {
-    switch (shape) { NVN_ROW_SHAPES_LIGHT(X) }
+    switch (shape) { NVN_RMS_FWD_SHAPES(X) }
   }
 #undef X
   return cudaErrorInvalidValue;
