@@ -317,8 +317,7 @@ constexpr int64_t kRmsHeldMinBytes = 32ll << 20;
   X(18, 256, 2, 1, 0, 12, 3)  X(19, 256, 2, 1, 0, 1, 3)   X(20, 128, 4, 1, 128, 12, 4)          \
   X(21, 128, 4, 1, 128, 1, 4) X(22, 128, 5, 1, 128, 12, 7) X(23, 320, 2, 1, 0, 1, 7)            \
   X(24, 256, 3, 1, 0, 12, 7)  X(25, 256, 3, 1, 0, 1, 7)   X(26, 256, 4, 1, 0, 12, 7)            \
-  X(27, 512, 2, 1, 0, 1, 7)   X(28, 512, 3, 1, 0, 12, 7)  X(29, 512, 3, 1, 0, 1, 7)             \
-  X(30, 512, 4, 1, 0, 12, 7)
+  X(27, 512, 2, 1, 0, 1, 7)   X(28, 512, 3, 1, 0, 12, 7)  X(29, 512, 4, 1, 0, 12, 7)
 // Accesses of less than 128 bits.  Against the LayerNorm table: f16 [12345, 1001] 20.3 -> 12.5 us
 // forward, 58 -> 34 us LayerNorm backward; bf16 [29363, 2347] residual 258 -> 122 us.  The widest
 // entry holds 16 values of four tensors per thread, too many with the dbeta sums (f16 [4000, 7031]

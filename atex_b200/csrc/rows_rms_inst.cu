@@ -118,6 +118,8 @@ template <int EPV, int TPR, int VPT, int RB, int MINB, int PF, int FORMS, int FO
 cudaError_t launch_one(const RowsResArgs& a, cudaStream_t s, bool dry, RowsPlan* plan) {
   if constexpr ((FORMS >> FORM & 1) == 0) {
     return cudaErrorInvalidValue;  // another form's entry
+  } else if constexpr (EPV != VecTraits<T>::kFull) {
+    return launch_exact<EPV, TPR, VPT, RB, true, MINB, PF, false, FORM>(a, s, dry, plan);
   } else {
     return a.D == static_cast<int64_t>(TPR) * VPT * EPV
                ? launch_exact<EPV, TPR, VPT, RB, true, MINB, PF, true, FORM>(a, s, dry, plan)

@@ -25,7 +25,7 @@ import torch
 from . import _lib
 from .nv_norm_ops import (InvalidArgumentError, LayerNormalization, _axis_list, _check, _dtype_code,
                           _grad_outputs, _like_output, _ln_dims, _on_device, _param, _remember,
-                          _require, _ws_bytes, fused_layer_norm_grad_op,
+                          _require, fused_layer_norm_grad_op,
                           fused_layer_norm_residual_op)
 
 __all__ = [
@@ -44,9 +44,26 @@ def _on_stream(index: int, fn, *args) -> int:
 
 
 def _scratch(like: torch.Tensor, nbytes: int) -> torch.Tensor:
-    """Workspace of one call, `like` a float32 tensor of the device.  nbytes is a multiple of 256.  From the caching allocator on the current stream, so that calls on
-    different streams and captured graphs never share one, and a captured graph owns its own."""
+    """Workspace of one call (nbytes a multiple of 256), on the device of the float32 tensor `like`.
+    From the caching allocator on the current stream, so that calls on different streams and
+    captured graphs never share one, and a captured graph owns its own."""
     return like.new_empty(nbytes // 4)
+
+
+class _Rows:
+    """A checked pair of x and scale: dtype code, rows, features, and the gradients' workspaces."""
+    __slots__ = ("code", "N", "D", "bytes")
+
+    def __init__(self, code, N, D):
+        self.code, self.N, self.D, self.bytes = code, N, D, {}
+
+    def workspace_bytes(self, fn_name: str, index: int) -> int:
+        """A size, asked for once with device `index` current."""
+        n = self.bytes.get(fn_name)
+        if n is None:
+            with torch.cuda.device(index):
+                n = self.bytes[fn_name] = int(getattr(_lib.load(), fn_name)(self.code, self.N, self.D))
+        return n
 
 
 # The checks of x and scale depend on their shapes and types alone; a small decoding step spends
@@ -54,11 +71,10 @@ def _scratch(like: torch.Tensor, nbytes: int) -> torch.Tensor:
 _rows_cache = {}
 
 
-def _rows(x, scale, axis):
-    """Checks x and scale against each other: (dtype code, N, D)."""
+def _rows(x, scale, axis) -> _Rows:
+    """Checks x and scale against each other."""
     try:
-        key = (x.shape, x.dtype, scale.shape, scale.dtype, axis)
-        return _rows_cache[key]
+        return _rows_cache[x.shape, x.dtype, scale.shape, scale.dtype, axis]
     except (KeyError, AttributeError, TypeError):
         pass
     _require(isinstance(x, torch.Tensor) and x.dim() > 0, "input must be at least 1-dimensional",
@@ -69,7 +85,7 @@ def _rows(x, scale, axis):
     N, D = _ln_dims(x, axis)
     _require(scale.numel() == D, "scale must have the same number of elements as the features "
              "of x, got ", scale.numel(), " and ", D)
-    return _remember(_rows_cache, (x.shape, x.dtype, scale.shape, scale.dtype, axis), (code, N, D))
+    return _remember(_rows_cache, (x.shape, x.dtype, scale.shape, scale.dtype, axis), _Rows(code, N, D))
 
 
 def _like_x(t, x, name):
@@ -78,6 +94,8 @@ def _like_x(t, x, name):
 
 
 def _saved(t, name, N):
+    if isinstance(t, torch.Tensor) and t.dtype == torch.float32 and t.shape == (N,):
+        return
     _param(t, name)
     _require(t.dim() == 1, name, " must be 1-dimensional", t)
     _require(t.numel() == N, name, " must have the same number of elements as the batches of x, got ",
@@ -108,14 +126,6 @@ def _one_output(like_numel, scale, out, name):
     return out
 
 
-def _on_device_bytes(index: int, fn_name: str, *args) -> int:
-    """A workspace size, asked for with device `index` current (and remembered)."""
-    if torch._C._cuda_getDevice() == index:
-        return _ws_bytes(fn_name, *args)
-    with torch.cuda.device(index):
-        return _ws_bytes(fn_name, *args)
-
-
 # ---------------------------------------------------------------------------
 # raw ops
 # ---------------------------------------------------------------------------
@@ -125,7 +135,8 @@ def fused_rms_norm_op(x, scale, axis: Iterable[int] = (-1,), epsilon: float = 0.
     (y, reserve_space_1), reserve_space_1 the per-row 1/sqrt(mean(x^2) + epsilon), float32 [N].
 
     `out` may be `x` itself; `out_stats` optionally supplies the reserve_space_1 buffer."""
-    code, N, D = _rows(x, scale, axis)
+    rows = _rows(x, scale, axis)
+    code, N, D = rows.code, rows.N, rows.D
     x, scale = _together((x, "x"), (scale, "scale"))
     y = _like_output(x, out, "out")
     inv = _one_output(N, scale, out_stats, "out_stats")
@@ -143,7 +154,8 @@ def fused_rms_norm_residual_op(x, residual, scale, axis: Iterable[int] = (-1,), 
 
     `out_sum` may be `x` or `residual` (the residual stream updated in place), `out` may be `x`
     or `residual`; the two must not be the same tensor."""
-    code, N, D = _rows(x, scale, axis)
+    rows = _rows(x, scale, axis)
+    code, N, D = rows.code, rows.N, rows.D
     _like_x(residual, x, "residual")
     x, residual, scale = _together((x, "x"), (residual, "residual"), (scale, "scale"))
     y = _like_output(x, out, "out")
@@ -158,7 +170,8 @@ def fused_rms_norm_residual_op(x, residual, scale, axis: Iterable[int] = (-1,), 
 
 
 def _rms_grad(dy, dsum, x, scale, inv, axis, out_grads, out):
-    code, N, D = _rows(x, scale, axis)
+    rows = _rows(x, scale, axis)
+    code, N, D = rows.code, rows.N, rows.D
     _like_x(dy, x, "y_backprop")
     _saved(inv, "reserve_space_1", N)
     if dsum is None:
@@ -170,7 +183,7 @@ def _rms_grad(dy, dsum, x, scale, inv, axis, out_grads, out):
     dx = _like_output(x, out, "out")
     dscale = torch.empty_like(scale) if out_grads is None else _one_output(D, scale, out_grads, "out_grads")
     index = x.get_device()
-    nbytes = _on_device_bytes(index, "nvn_rms_bwd_workspace_bytes", code, N, D)
+    nbytes = rows.workspace_bytes("nvn_rms_bwd_workspace_bytes", index)
     ws = _scratch(scale, nbytes)
     st = _on_stream(index, _lib.load().nvn_rms_bwd, code, dy.data_ptr(), 0 if dsum is None else dsum.data_ptr(),
                     x.data_ptr(), scale.data_ptr(), inv.data_ptr(), N, D, dx.data_ptr(), dscale.data_ptr(),
@@ -208,7 +221,8 @@ def fused_layer_norm_residual_grad_op(y_backprop, sum_backprop, s, scale, reserv
     offset_backprop).  `s` is the op's sum output, sum_backprop the gradient that reaches it
     from the residual stream; x_backprop is the gradient of x and of residual.  `out` may be
     sum_backprop; `out_grads` optionally supplies the (scale_backprop, offset_backprop) pair."""
-    code, N, D = _rows(s, scale, axis)
+    rows = _rows(s, scale, axis)
+    code, N, D = rows.code, rows.N, rows.D
     _like_x(y_backprop, s, "y_backprop")
     _like_x(sum_backprop, s, "sum_backprop")
     _saved(reserve_space_1, "reserve_space_1", N)
@@ -219,7 +233,7 @@ def fused_layer_norm_residual_grad_op(y_backprop, sum_backprop, s, scale, reserv
     dx = _like_output(x, out, "out")
     dscale, doffset = _grad_outputs(scale, out_grads)
     index = x.get_device()
-    nbytes = _on_device_bytes(index, "nvn_ln_bwd_residual_workspace_bytes", code, N, D)
+    nbytes = rows.workspace_bytes("nvn_ln_bwd_residual_workspace_bytes", index)
     ws = _scratch(scale, nbytes)
     st = _on_stream(index, _lib.load().nvn_ln_bwd_residual, code, dy.data_ptr(), dsum.data_ptr(), x.data_ptr(),
                     scale.data_ptr(), mean.data_ptr(), inv.data_ptr(), N, D, dx.data_ptr(), dscale.data_ptr(),
