@@ -39,10 +39,13 @@
 namespace nvn {
 
 // Threads per CTA, and the CTAs per SM that the registers are limited for: with two rows at once
-// 5 (backward 3) small CTAs of up to 102 (168) registers; with one row 3 (2) of 80 (128).  Small
+// 5 (backward 4, with offsets 3) small CTAs of up to 102 (128, 168) registers; with one row 3 (2)
+// of 80 (128).  Small
 // CTAs for one row were slower (f32 [3, 1025, 10+2, 80] gradient 17.5 -> 20.0 us).
 __host__ __device__ constexpr int head_block(int rows) { return rows > 1 ? 128 : 256; }
-__host__ __device__ constexpr int head_ctas(bool bwd, int rows) { return bwd ? (rows > 1 ? 3 : 2) : (rows > 1 ? 5 : 3); }
+__host__ __device__ constexpr int head_ctas(bool bwd, int rows, int norm) {
+  return bwd ? (rows > 1 ? (norm == 2 ? 3 : 4) : 2) : (rows > 1 ? 5 : 3);
+}
 
 // n / d for n < 2^31 by a multiplication: with 2^(s-1) < d <= 2^s and m = ceil(2^(31+s) / d),
 // m d - 2^(31+s) < d <= 2^s, so floor(n m / 2^(31+s)) is exact.
@@ -221,6 +224,11 @@ __device__ __forceinline__ void head_rotate(E (&v)[R][SPT][2][NE], const float* 
   }
 }
 
+// 16 bytes from global to shared memory; cp.async.wait_all of the same thread makes them visible.
+__device__ __forceinline__ void head_copy16(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+}
+
 // Where a row (the first of R) is read, and where it goes: null for one that is none.
 struct alignas(16) HeadSource {
   const void* x;
@@ -238,7 +246,7 @@ struct alignas(16) HeadTarget {
 // FULL: lanes per head when the head fills them exactly and every element is rotated (head_dim 64,
 // 128 or 256, no predicates and a fixed reduction); 0: any head.
 template <typename T, int V, int NORM, bool IL, bool BWD, int FULL, int R>
-__global__ void __launch_bounds__(head_block(R), head_ctas(BWD, R)) head_kernel(const HeadArgs a) {
+__global__ void __launch_bounds__(head_block(R), head_ctas(BWD, R, NORM)) head_kernel(const HeadArgs a) {
   constexpr int BLOCK = head_block(R);
   constexpr int SPT = HeadTraits<V>::SPT;
   using M = typename MathSel<V>::M;
@@ -247,12 +255,18 @@ __global__ void __launch_bounds__(head_block(R), head_ctas(BWD, R)) head_kernel(
   using P = Pack<T, V>;
   constexpr int NV = NORM;                         // parameter vectors per part
   constexpr bool READ_X = !BWD || NORM != 0;       // without a norm the gradient needs no x
-  // dynamic shared memory: gradient sums [2][NV][16][threads] (backward), three buffers of row
+  // The next rows wait in registers, or - two rows of two tensors would take 32 - in 16-byte slots
+  // of shared memory that the thread copies to and reads back itself.
+  constexpr bool ASYNC = BWD && R > 1;
+  static_assert(!ASYNC || sizeof(P) == 16, "cp.async moves 16 bytes here");
+  // dynamic shared memory: gradient sums [2][NV][16][threads] (backward), the threads' slots
+  // [R][SPT][2][x, dy][threads] (two rows backward), three buffers of row
   // addresses [rows] (where x and dy are read; where the result goes, and the row's angles),
   // parameters [2][NV][hd4], three buffers of angles [tile][pstride]
   extern __shared__ __align__(16) float head_smem[];
   float* const sums = head_smem;
-  HeadSource* const sources = reinterpret_cast<HeadSource*>(sums + (BWD ? 2 * NV * 16 * BLOCK : 0));
+  P* const slots = reinterpret_cast<P*>(sums + (BWD ? 2 * NV * 16 * BLOCK : 0)) + threadIdx.x;
+  HeadSource* const sources = reinterpret_cast<HeadSource*>(slots - threadIdx.x + (ASYNC ? R * SPT * 4 * BLOCK : 0));
   HeadTarget* const targets = reinterpret_cast<HeadTarget*>(sources + 3 * a.rows);
   float* const par = reinterpret_cast<float*>(targets + 3 * a.rows);
   float* const tables = par + 2 * NV * a.hd4;
@@ -352,15 +366,26 @@ __global__ void __launch_bounds__(head_block(R), head_ctas(BWD, R)) head_kernel(
   };
 
   P xr[R][SPT][2], dr[R][SPT][2];
+  auto slot = [&](int r, int i, int k, int tensor) -> P* {
+    return slots + (((r * SPT + i) * 2 + k) * 2 + tensor) * BLOCK;
+  };
   auto clear = [&]() {
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int i = 0; i < SPT; ++i)
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+        for (int k = 0; k < 2; ++k) {
+          P zero;
 #pragma unroll
-          for (int e = 0; e < V; ++e) xr[r][i][k].v[e] = dr[r][i][k].v[e] = Cvt<T>::from_f32(0.f);
+          for (int e = 0; e < V; ++e) zero.v[e] = Cvt<T>::from_f32(0.f);
+          if constexpr (ASYNC) {
+            *slot(r, i, k, 0) = zero;
+            *slot(r, i, k, 1) = zero;
+          } else {
+            xr[r][i][k] = dr[r][i][k] = zero;
+          }
+        }
   };
   // Starts the loads of a group's rows.
   auto fetch = [&](const HeadSource src, int part) {
@@ -374,15 +399,25 @@ __global__ void __launch_bounds__(head_block(R), head_ctas(BWD, R)) head_kernel(
 #pragma unroll
           for (int k = 0; k < 2; ++k)
             if (valid[i][k]) {
-              if constexpr (READ_X) xr[r][i][k] = load_stream<T, V>(xp, col[i][k]);
-              if constexpr (BWD) dr[r][i][k] = load_stream<T, V>(dp, col[i][k]);
+              if constexpr (ASYNC) {
+                if constexpr (READ_X) head_copy16(slot(r, i, k, 0), xp + col[i][k]);
+                head_copy16(slot(r, i, k, 1), dp + col[i][k]);
+              } else {
+                if constexpr (READ_X) xr[r][i][k] = load_stream<T, V>(xp, col[i][k]);
+                if constexpr (BWD) dr[r][i][k] = load_stream<T, V>(dp, col[i][k]);
+              }
             }
       }
-    } else if constexpr (BWD) {
-      clear();   // a group without a row adds nothing to the parameter sums
+    }
+    if constexpr (BWD) {
+      // a group without a row adds nothing to the parameter sums (a branch of the whole warp,
+      // which hardly any warp takes)
+      if (__any_sync(0xffffffffu, src.x == nullptr)) {
+        if (src.x == nullptr) clear();
+      }
     }
   };
-  clear();
+  if constexpr (!ASYNC) clear();   // vectors that no row fills stay zero
 
   auto fill_parameters = [&]() {
     if constexpr (NV > 0) {
@@ -459,14 +494,20 @@ __global__ void __launch_bounds__(head_block(R), head_ctas(BWD, R)) head_kernel(
 #pragma unroll 1
       for (int step = part == 0 ? 0 : q_end; step < stop; ++step) {
         E x[R][SPT][2][NE], d[R][SPT][2][NE];
+        if constexpr (ASYNC) asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
           for (int i = 0; i < SPT; ++i)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-              if constexpr (READ_X) unpack<T, V>(xr[r][i][k], x[r][i][k]);
-              if constexpr (BWD) unpack<T, V>(dr[r][i][k], d[r][i][k]);
+              if constexpr (ASYNC) {
+                if constexpr (READ_X) unpack<T, V>(*slot(r, i, k, 0), x[r][i][k]);
+                unpack<T, V>(*slot(r, i, k, 1), d[r][i][k]);
+              } else {
+                if constexpr (READ_X) unpack<T, V>(xr[r][i][k], x[r][i][k]);
+                if constexpr (BWD) unpack<T, V>(dr[r][i][k], d[r][i][k]);
+              }
             }
         // the group's next rows, of this tile or the next
         if (step + 1 < end) {

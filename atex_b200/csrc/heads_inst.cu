@@ -61,7 +61,7 @@ cudaError_t launch_kernel(HeadArgs a, cudaStream_t s, bool dry_run, HeadPlan* pl
   }
   const int hq = a.part[0].heads, hk = a.parts > 1 ? a.part[1].heads : 0;
   const int most_steps = kMaxRows / R / groups < 8 ? kMaxRows / R / groups : 8;
-  const int64_t ctas = static_cast<int64_t>(device_sm_count()) * head_ctas(kBwd, R);
+  const int64_t ctas = static_cast<int64_t>(device_sm_count()) * head_ctas(kBwd, R, NORM);
   int64_t tile = static_cast<int64_t>(most_steps) * groups / (hq + hk);
   if (tile > kTableBytes / (3 * 4 * a.pstride)) tile = kTableBytes / (3 * 4 * a.pstride);
   if (tile < 1) tile = 1;
@@ -76,12 +76,14 @@ cudaError_t launch_kernel(HeadArgs a, cudaStream_t s, bool dry_run, HeadPlan* pl
   a.pieces = (a.all_steps + a.steps - 1) / a.steps;
   a.tiles = blocks * a.pieces;
   a.rows = a.steps * groups;
-  const size_t fixed = static_cast<size_t>(2 * NV * a.hd4 + (kBwd ? 2 * NV * 16 * BLOCK : 0)) * 4;
+  constexpr size_t kSlots = kBwd && R > 1 ? R * SPT * 4 * BLOCK * 16 : 0;
+  const size_t fixed =
+      static_cast<size_t>(2 * NV * a.hd4 + (kBwd ? 2 * NV * 16 * BLOCK : 0)) * 4 + kSlots;
   const size_t smem = fixed + static_cast<size_t>(3) * (32 * a.rows + 4 * a.tile * a.pstride);
   static std::atomic<uint64_t> prepared{0};
   cudaError_t e = once_per_device(prepared, [&]() -> cudaError_t {
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                kTableBytes + 3 * 32 * (kMaxRows + 2 * BLOCK) +
+                                static_cast<int>(kSlots) + kTableBytes + 3 * 32 * (kMaxRows + 2 * BLOCK) +
                                     (2 * NV * 512 + (kBwd ? 2 * NV * 16 * BLOCK : 0)) * 4);
   });
   if (e != cudaSuccess) return e;
@@ -139,7 +141,7 @@ cudaError_t launch(HeadArgs& a, cudaStream_t s, bool dry, HeadPlan* plan) {
         const int hq = a.part[0].heads, hk = a.parts > 1 ? a.part[1].heads : 0;
         const int groups = head_block(1) / (a.hd / 16);
         if (hq % 2 == 0 && hk % 2 == 0 &&
-            a.N * (hq + hk) >= static_cast<int64_t>(device_sm_count()) * head_ctas(kBwd, 1) * groups)
+            a.N * (hq + hk) >= static_cast<int64_t>(device_sm_count()) * head_ctas(kBwd, 1, NORM) * groups)
           return launch_full<V, NORM, IL, 2>(a, s, dry, plan);
       }
       return launch_full<V, NORM, IL, 1>(a, s, dry, plan);
