@@ -39,12 +39,13 @@
 namespace nvn {
 
 // Threads per CTA, and the CTAs per SM that the registers are limited for: with two rows at once
-// 5 (backward 4, with offsets 3) small CTAs of up to 102 (128, 168) registers; with one row 3 (2)
-// of 80 (128).  Small
+// 5, with offsets 4, (backward 4, with offsets or padding 3) small CTAs of up to 102, 128 (128,
+// 168) registers; with one row 3 (2) of 80 (128).  Spilling to fit a fourth cost more than it gave (88 -> 115 us).  Small
 // CTAs for one row were slower (f32 [3, 1025, 10+2, 80] gradient 17.5 -> 20.0 us).
 __host__ __device__ constexpr int head_block(int rows) { return rows > 1 ? 128 : 256; }
-__host__ __device__ constexpr int head_ctas(bool bwd, int rows, int norm) {
-  return bwd ? (rows > 1 ? (norm == 2 ? 3 : 4) : 2) : (rows > 1 ? 5 : 3);
+__host__ __device__ constexpr int head_ctas(bool bwd, int rows, int norm, bool pad) {
+  return bwd ? (rows > 1 ? (norm == 2 || (norm == 1 && pad) ? 3 : 4) : 2)
+             : (rows > 1 ? (norm == 2 ? 4 : 5) : 3);
 }
 
 // n / d for n < 2^31 by a multiplication: with 2^(s-1) < d <= 2^s and m = ceil(2^(31+s) / d),
@@ -105,8 +106,9 @@ __device__ __forceinline__ float neg(float v) { return -v; }
 
 // (a, b) -> (a cos - b sin, a sin + b cos), turned back for SIGN < 0.
 // `left` is the number of the slot's pairs that are rotated, for interleaved pairs whose rotated
-// range ends inside a vector (an infinity beside it must not meet a sine of zero).
-template <int V, bool IL, int SIGN, typename E, int NE>
+// range ends inside a vector (an infinity beside it must not meet a sine of zero); with WHOLE a
+// slot is rotated or not.
+template <int V, bool IL, int SIGN, bool WHOLE, typename E, int NE>
 __device__ __forceinline__ void head_turn(E (&a)[NE], E (&b)[NE], const float (&c)[V],
                                           const float (&sn)[V], bool rot_a, bool rot_b, int left) {
   using M = typename MathSel<V>::M;
@@ -132,15 +134,21 @@ __device__ __forceinline__ void head_turn(E (&a)[NE], E (&b)[NE], const float (&
       const float cc = c[e], ss = SIGN < 0 ? -sn[e] : sn[e];
       const float u = fmaf(v.x, cc, -(v.y * ss));
       const float w = fmaf(v.x, ss, v.y * cc);
-      if (e < left) v = make_float2(u, w);
+      if (WHOLE || e < left) v = make_float2(u, w);
     };
     if (rot_a) {
 #pragma unroll
       for (int e = 0; e < NE; ++e) turn(a[e], e);
-    }
-    if (rot_b) {
+      if constexpr (WHOLE) {
 #pragma unroll
-      for (int e = 0; e < NE; ++e) turn(b[e], NE + e);
+        for (int e = 0; e < NE; ++e) turn(b[e], NE + e);
+      }
+    }
+    if constexpr (!WHOLE) {
+      if (rot_b) {
+#pragma unroll
+        for (int e = 0; e < NE; ++e) turn(b[e], NE + e);
+      }
     }
   }
 }
@@ -210,17 +218,17 @@ __device__ __forceinline__ void head_sums_store(float* p, int j, const typename 
 
 // Turns every slot of R rows of one token by its angles.
 template <int V, bool IL, int SIGN, int FULL, int R, int SPT, typename E, int NE>
-__device__ __forceinline__ void head_rotate(E (&v)[R][SPT][2][NE], const float* tab, int lane, int tph,
-                                            const bool (&rot)[SPT][2], int pairs) {
+__device__ __forceinline__ void head_rotate(E (&v)[R][SPT][2][NE], const float* tab, int nslots,
+                                            const int (&slot_of)[SPT], const bool (&rot)[SPT][2], int pairs) {
 #pragma unroll
   for (int i = 0; i < SPT; ++i) {
     float c[V], s[V];
-    head_table_read<V>(tab, false, lane + i * tph, SPT * tph, c);
-    head_table_read<V>(tab, true, lane + i * tph, SPT * tph, s);
+    head_table_read<V>(tab, false, slot_of[i], nslots, c);
+    head_table_read<V>(tab, true, slot_of[i], nslots, s);
 #pragma unroll
     for (int r = 0; r < R; ++r)
-      head_turn<V, IL, SIGN>(v[r][i][0], v[r][i][1], c, s, rot[i][0], rot[i][1],
-                             FULL != 0 ? V : pairs - (lane + i * tph) * V);
+      head_turn<V, IL, SIGN, FULL != 0>(v[r][i][0], v[r][i][1], c, s, rot[i][0], rot[i][1],
+                                        pairs - slot_of[i] * V);
   }
 }
 
@@ -243,10 +251,13 @@ struct alignas(16) HeadTarget {
 // NORM: 0 none, 1 root mean square, 2 mean and variance.  IL: interleaved pairs.
 // R: rows a group works on at once, neighbouring heads of one token: they share its angles and the
 // parameters, and their reductions overlap.
-// FULL: lanes per head when the head fills them exactly and every element is rotated (head_dim 64,
-// 128 or 256, no predicates and a fixed reduction); 0: any head.
-template <typename T, int V, int NORM, bool IL, bool BWD, int FULL, int R>
-__global__ void __launch_bounds__(head_block(R), head_ctas(BWD, R, NORM)) head_kernel(const HeadArgs a) {
+// FULL: lanes per head (4, 8, 16) of heads that are whole slots, rotated slot by slot (in 16 bits
+// head_dim a multiple of 16 up to 256 and pairs of 8): the reduction is fixed.  Without PAD the
+// head fills its lanes and is rotated whole; with PAD lanes behind its last slot repeat that slot -
+// only their sums and stores are left out, where predicates around every access cost a tenth of
+// the time.  0: any head.
+template <typename T, int V, int NORM, bool IL, bool BWD, int FULL, bool PAD, int R>
+__global__ void __launch_bounds__(head_block(R), head_ctas(BWD, R, NORM, PAD)) head_kernel(const HeadArgs a) {
   constexpr int BLOCK = head_block(R);
   constexpr int SPT = HeadTraits<V>::SPT;
   using M = typename MathSel<V>::M;
@@ -286,15 +297,20 @@ __global__ void __launch_bounds__(head_block(R), head_ctas(BWD, R, NORM)) head_k
   griddep_wait();
   // this thread's vectors
   int col[SPT][2];
-  bool valid[SPT][2], rot[SPT][2];
+  int slot_of[SPT];
+  bool valid[SPT][2], rot[SPT][2], ok[SPT];
 #pragma unroll
   for (int i = 0; i < SPT; ++i) {
-    const int s = lane + i * tph;
+    int s = lane + i * tph;
+    ok[i] = !PAD || 2 * s < vectors;
+    if (!ok[i]) s = vectors / 2 - 1;
+    slot_of[i] = s;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       col[i][h] = head_col<V, IL>(s, h, pairs);
       valid[i][h] = FULL != 0 || (!IL && s * V < pairs) || 2 * s + h < vectors;
-      rot[i][h] = FULL != 0 || ((!IL || V == 1) ? s * V < pairs : (2 * s + h) * V < 2 * pairs);
+      rot[i][h] = (FULL != 0 && !PAD) ||
+                  ((FULL != 0 || !IL || V == 1) ? s * V < pairs : (2 * s + h) * V < 2 * pairs);
     }
   }
 
@@ -417,7 +433,18 @@ __global__ void __launch_bounds__(head_block(R), head_ctas(BWD, R, NORM)) head_k
       }
     }
   };
-  if constexpr (!ASYNC) clear();   // vectors that no row fills stay zero
+  // vectors that no row fills stay zero
+  if constexpr (!ASYNC) {
+    clear();
+  } else if constexpr (FULL == 0) {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int i = 0; i < SPT; ++i)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          if (!valid[i][k]) *slot(r, i, k, 0) = *slot(r, i, k, 1) = P{};
+  }
 
   auto fill_parameters = [&]() {
     if constexpr (NV > 0) {
@@ -518,19 +545,21 @@ __global__ void __launch_bounds__(head_block(R), head_ctas(BWD, R, NORM)) head_k
         const HeadTarget dst = targets[buf * a.rows + (step << glog) + group];
         const bool on = dst.out != nullptr;
         const float* tt = tab + dst.angles;
-        if constexpr (BWD) head_rotate<V, IL, -1, FULL, R>(d, tt, lane, tph, rot, pairs);
+        if constexpr (BWD) head_rotate<V, IL, -1, FULL, R>(d, tt, nslots, slot_of, rot, pairs);
         if constexpr (NORM == 2) {
           float m[R];
 #pragma unroll
           for (int r = 0; r < R; ++r) {
-            E acc = M::bcast(0.f);
+            m[r] = 0.f;
 #pragma unroll
-            for (int i = 0; i < SPT; ++i)
+            for (int i = 0; i < SPT; ++i) {
+              E acc = M::bcast(0.f);
 #pragma unroll
               for (int k = 0; k < 2; ++k)
 #pragma unroll
                 for (int e = 0; e < NE; ++e) acc = M::add(acc, x[r][i][k][e]);
-            m[r] = M::hsum(acc);
+              if (ok[i]) m[r] += M::hsum(acc);
+            }
           }
           head_reduce<FULL>(m, tph);
 #pragma unroll
@@ -551,11 +580,13 @@ __global__ void __launch_bounds__(head_block(R), head_ctas(BWD, R, NORM)) head_k
           float red[NR * R];
 #pragma unroll
           for (int r = 0; r < R; ++r) {
-            E acc[NR];
 #pragma unroll
-            for (int k = 0; k < NR; ++k) acc[k] = M::bcast(0.f);
+            for (int k = 0; k < NR; ++k) red[r * NR + k] = 0.f;
 #pragma unroll
-            for (int i = 0; i < SPT; ++i)
+            for (int i = 0; i < SPT; ++i) {
+              E acc[NR];
+#pragma unroll
+              for (int k = 0; k < NR; ++k) acc[k] = M::bcast(0.f);
 #pragma unroll
               for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -568,8 +599,9 @@ __global__ void __launch_bounds__(head_block(R), head_ctas(BWD, R, NORM)) head_k
                   }
                 }
 #pragma unroll
-            for (int k = 0; k < NR; ++k)
-              red[r * NR + k] = M::hsum(acc[k]) * a.inv_hd;  // shares of means: no overflow in the sum
+              for (int k = 0; k < NR; ++k)   // shares of means: no overflow in the sum
+                if (ok[i]) red[r * NR + k] += M::hsum(acc[k]) * a.inv_hd;
+            }
           }
           head_reduce<FULL>(red, tph);
 #pragma unroll
@@ -610,7 +642,7 @@ __global__ void __launch_bounds__(head_block(R), head_ctas(BWD, R, NORM)) head_k
             }
           }
         }
-        if constexpr (!BWD) head_rotate<V, IL, 1, FULL, R>(x, tt, lane, tph, rot, pairs);
+        if constexpr (!BWD) head_rotate<V, IL, 1, FULL, R>(x, tt, nslots, slot_of, rot, pairs);
         if (on) {
 #pragma unroll
           for (int r = 0; r < R; ++r) {
@@ -619,7 +651,7 @@ __global__ void __launch_bounds__(head_block(R), head_ctas(BWD, R, NORM)) head_k
             for (int i = 0; i < SPT; ++i)
 #pragma unroll
               for (int k = 0; k < 2; ++k)
-                if (valid[i][k]) {
+                if (valid[i][k] && ok[i]) {
                   if constexpr (BWD) {
                     store_stream<T, V>(op, col[i][k], repack<T, V>(d[r][i][k]));
                   } else {

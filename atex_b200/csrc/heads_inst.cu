@@ -32,9 +32,9 @@ constexpr int kTableBytes = 48 * 1024;   // most that a tile's angles may take
 
 inline int round4(int v) { return (v + 3) / 4 * 4; }
 
-template <int V, int NORM, bool IL, int FULL, int R>
+template <int V, int NORM, bool IL, int FULL, bool PAD, int R>
 cudaError_t launch_kernel(HeadArgs a, cudaStream_t s, bool dry_run, HeadPlan* plan) {
-  auto kernel = head_kernel<T, V, NORM, IL, kBwd, FULL, R>;
+  auto kernel = head_kernel<T, V, NORM, IL, kBwd, FULL, PAD, R>;
   constexpr int BLOCK = head_block(R);
   constexpr int SPT = HeadTraits<V>::SPT;
   constexpr int NV = NORM;
@@ -61,9 +61,16 @@ cudaError_t launch_kernel(HeadArgs a, cudaStream_t s, bool dry_run, HeadPlan* pl
   }
   const int hq = a.part[0].heads, hk = a.parts > 1 ? a.part[1].heads : 0;
   const int most_steps = kMaxRows / R / groups < 8 ? kMaxRows / R / groups : 8;
-  const int64_t ctas = static_cast<int64_t>(device_sm_count()) * head_ctas(kBwd, R, NORM);
+  const int64_t ctas = static_cast<int64_t>(device_sm_count()) * head_ctas(kBwd, R, NORM, PAD);
   int64_t tile = static_cast<int64_t>(most_steps) * groups / (hq + hk);
-  if (tile > kTableBytes / (3 * 4 * a.pstride)) tile = kTableBytes / (3 * 4 * a.pstride);
+  // what one CTA's tables may take so that the registers, and not they, set the CTAs per SM
+  constexpr size_t kSlots = kBwd && R > 1 ? R * SPT * 4 * BLOCK * 16 : 0;
+  const size_t fixed =
+      static_cast<size_t>(2 * NV * a.hd4 + (kBwd ? 2 * NV * 16 * BLOCK : 0)) * 4 + kSlots;
+  int64_t room = (227 * 1024) / head_ctas(kBwd, R, NORM, PAD) - 1024 - static_cast<int64_t>(fixed) -
+                 3 * 32 * (most_steps + 2) * groups;
+  if (room > kTableBytes) room = kTableBytes;
+  if (tile > room / (3 * 4 * a.pstride)) tile = room / (3 * 4 * a.pstride);
   if (tile < 1) tile = 1;
   const int64_t waves = (a.N + tile * ctas - 1) / (tile * ctas);
   tile = (a.N + waves * ctas - 1) / (waves * ctas);
@@ -76,9 +83,6 @@ cudaError_t launch_kernel(HeadArgs a, cudaStream_t s, bool dry_run, HeadPlan* pl
   a.pieces = (a.all_steps + a.steps - 1) / a.steps;
   a.tiles = blocks * a.pieces;
   a.rows = a.steps * groups;
-  constexpr size_t kSlots = kBwd && R > 1 ? R * SPT * 4 * BLOCK * 16 : 0;
-  const size_t fixed =
-      static_cast<size_t>(2 * NV * a.hd4 + (kBwd ? 2 * NV * 16 * BLOCK : 0)) * 4 + kSlots;
   const size_t smem = fixed + static_cast<size_t>(3) * (32 * a.rows + 4 * a.tile * a.pstride);
   static std::atomic<uint64_t> prepared{0};
   cudaError_t e = once_per_device(prepared, [&]() -> cudaError_t {
@@ -126,28 +130,33 @@ cudaError_t launch_kernel(HeadArgs a, cudaStream_t s, bool dry_run, HeadPlan* pl
 
 template <int V, int NORM, bool IL, int R>
 cudaError_t launch_full(HeadArgs& a, cudaStream_t s, bool dry, HeadPlan* plan) {
-  if (a.hd == 64) return launch_kernel<V, NORM, IL, 4, R>(a, s, dry, plan);
-  if (a.hd == 128) return launch_kernel<V, NORM, IL, 8, R>(a, s, dry, plan);
-  return launch_kernel<V, NORM, IL, 16, R>(a, s, dry, plan);
+  const bool pad = (a.hd != 64 && a.hd != 128 && a.hd != 256) || 2 * a.pairs != a.hd;
+#define NVN_HEADS(FULL)                                                      \
+  return pad ? launch_kernel<V, NORM, IL, FULL, true, R>(a, s, dry, plan)    \
+             : launch_kernel<V, NORM, IL, FULL, false, R>(a, s, dry, plan)
+  if (a.hd <= 64) NVN_HEADS(4);
+  if (a.hd <= 128) NVN_HEADS(8);
+  NVN_HEADS(16);
+#undef NVN_HEADS
 }
 
 template <int V, int NORM, bool IL>
 cudaError_t launch(HeadArgs& a, cudaStream_t s, bool dry, HeadPlan* plan) {
   if constexpr (V == VecTraits<T>::kFull) {
-    if (2 * a.pairs == a.hd && (a.hd == 64 || a.hd == 128 || a.hd == 256)) {
-      // two heads at once in 16 bits, when they pair up and there is work for every CTA; fp32 rows
-      // are twice as long and would not fit in the registers
+    if (a.hd > 32 && a.hd <= 256 && a.hd % (2 * V) == 0 && a.pairs % V == 0) {
+      // Two heads at once in 16 bits, when they pair up and there is work for every CTA; fp32
+      // rows are twice as long and would not fit in the registers.
       if constexpr (sizeof(T) == 2) {
         const int hq = a.part[0].heads, hk = a.parts > 1 ? a.part[1].heads : 0;
-        const int groups = head_block(1) / (a.hd / 16);
+        const int groups = head_block(1) / (a.hd <= 64 ? 4 : (a.hd <= 128 ? 8 : 16));
         if (hq % 2 == 0 && hk % 2 == 0 &&
-            a.N * (hq + hk) >= static_cast<int64_t>(device_sm_count()) * head_ctas(kBwd, 1, NORM) * groups)
+            a.N * (hq + hk) >= static_cast<int64_t>(device_sm_count()) * head_ctas(kBwd, 1, NORM, false) * groups)
           return launch_full<V, NORM, IL, 2>(a, s, dry, plan);
       }
       return launch_full<V, NORM, IL, 1>(a, s, dry, plan);
     }
   }
-  return launch_kernel<V, NORM, IL, 0, 1>(a, s, dry, plan);
+  return launch_kernel<V, NORM, IL, 0, false, 1>(a, s, dry, plan);
 }
 
 template <int V>
