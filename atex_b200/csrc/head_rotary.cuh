@@ -16,9 +16,10 @@
 // elements each, as SPT slots of two vectors (A, B) of V elements:
 //   split pairs (p, p + pairs):   slot s < pairs / V is A = [sV, sV + V), B = the same + pairs,
 //                                 so a thread holds both halves of its V pairs
-//   interleaved (2p, 2p + 1):     slot s is the 2V elements from 2sV on, V pairs as well
+//   interleaved (2p, 2p + 1):     slot s is the 2V elements from 2sV on, V pairs as well; a head of
+//                                 whole slots (FULL below) takes A = [sV, sV + V) and B half a head
+//                                 behind it, so that neighbouring lanes copy neighbouring vectors
 //   behind the rotated elements a slot is 2V plain elements.
-// In every form slot s turns by the V angles from pair sV on.
 //
 // A CTA takes tiles: a block of consecutive tokens with all their heads, queries and keys - or, when
 // a token has more rows than a tile, or tokens are few, a piece of the block's rows.  The angles of a
@@ -62,18 +63,24 @@ struct HeadTraits {
 };
 
 // Element column of vector `half` of slot s.
-template <int V, bool IL>
-__device__ __forceinline__ int head_col(int s, int half, int pairs) {
+template <int V, bool IL, int FULL>
+__device__ __forceinline__ int head_col(int s, int half, int pairs, int hd) {
+  if (IL && FULL != 0) return s * V + half * (hd / 2);
   if (!IL && s * V < pairs) return half == 0 ? s * V : s * V + pairs;
   return (2 * s + half) * V;
 }
 
 // Angle table of one token: [cos, sin][chunk][slot][CW], so that neighbouring lanes read
 // neighbouring 16-byte words.
-template <int V>
-__device__ __forceinline__ int head_table_at(int p, bool sine, int nslots) {
+template <int V, bool IL, int FULL>
+__device__ __forceinline__ int head_table_at(int p, bool sine, int nslots, int hd) {
   constexpr int CW = HeadTraits<V>::CW, CHUNKS = HeadTraits<V>::CHUNKS;
-  const int s = p / V, e = p % V;
+  int s = p / V, e = p % V;
+  if constexpr (IL && FULL != 0) {   // vector v = 2p / V is slot v's A, or slot (v - half)'s B
+    const int v = p / (V / 2), half = hd / (2 * V);
+    s = v < half ? v : v - half;
+    e = p % (V / 2) + (v < half ? 0 : V / 2);
+  }
   return (((sine ? CHUNKS : 0) + e / CW) * nslots + s) * CW + e % CW;
 }
 
@@ -107,7 +114,7 @@ __device__ __forceinline__ float neg(float v) { return -v; }
 // (a, b) -> (a cos - b sin, a sin + b cos), turned back for SIGN < 0.
 // `left` is the number of the slot's pairs that are rotated, for interleaved pairs whose rotated
 // range ends inside a vector (an infinity beside it must not meet a sine of zero); with WHOLE a
-// slot is rotated or not.
+// vector is rotated or not.
 template <int V, bool IL, int SIGN, bool WHOLE, typename E, int NE>
 __device__ __forceinline__ void head_turn(E (&a)[NE], E (&b)[NE], const float (&c)[V],
                                           const float (&sn)[V], bool rot_a, bool rot_b, int left) {
@@ -139,16 +146,10 @@ __device__ __forceinline__ void head_turn(E (&a)[NE], E (&b)[NE], const float (&
     if (rot_a) {
 #pragma unroll
       for (int e = 0; e < NE; ++e) turn(a[e], e);
-      if constexpr (WHOLE) {
-#pragma unroll
-        for (int e = 0; e < NE; ++e) turn(b[e], NE + e);
-      }
     }
-    if constexpr (!WHOLE) {
-      if (rot_b) {
+    if (rot_b) {
 #pragma unroll
-        for (int e = 0; e < NE; ++e) turn(b[e], NE + e);
-      }
+      for (int e = 0; e < NE; ++e) turn(b[e], NE + e);
     }
   }
 }
@@ -307,10 +308,10 @@ __global__ void __launch_bounds__(head_block(R), head_ctas(BWD, R, NORM, PAD)) h
     slot_of[i] = s;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      col[i][h] = head_col<V, IL>(s, h, pairs);
+      col[i][h] = head_col<V, IL, FULL>(s, h, pairs, a.hd);
       valid[i][h] = FULL != 0 || (!IL && s * V < pairs) || 2 * s + h < vectors;
       rot[i][h] = (FULL != 0 && !PAD) ||
-                  ((FULL != 0 || !IL || V == 1) ? s * V < pairs : (2 * s + h) * V < 2 * pairs);
+                  ((!IL || V == 1) ? s * V < pairs : col[i][h] < 2 * pairs);
     }
   }
 
@@ -376,8 +377,8 @@ __global__ void __launch_bounds__(head_block(R), head_ctas(BWD, R, NORM, PAD)) h
         turns -= rint(turns);
         sincospif(2.f * static_cast<float>(turns), &s, &c);
       }
-      tab[lt * a.pstride + head_table_at<V>(p, false, nslots)] = c;
-      tab[lt * a.pstride + head_table_at<V>(p, true, nslots)] = s;
+      tab[lt * a.pstride + head_table_at<V, IL, FULL>(p, false, nslots, a.hd)] = c;
+      tab[lt * a.pstride + head_table_at<V, IL, FULL>(p, true, nslots, a.hd)] = s;
     }
   };
 
@@ -455,10 +456,11 @@ __global__ void __launch_bounds__(head_block(R), head_ctas(BWD, R, NORM, PAD)) h
       }
     }
     // slots behind the rotated pairs turn by nothing
-    for (int i = tid; i < 3 * a.tile * (nslots * V - pairs); i += BLOCK) {
-      const int row = i / (nslots * V - pairs), p = pairs + i - row * (nslots * V - pairs);
-      tables[row * a.pstride + head_table_at<V>(p, false, nslots)] = 1.f;
-      tables[row * a.pstride + head_table_at<V>(p, true, nslots)] = 0.f;
+    const int plain = (FULL != 0 ? a.hd / 2 : nslots * V) - pairs;
+    for (int i = tid; i < 3 * a.tile * plain; i += BLOCK) {
+      const int row = i / plain, p = pairs + i - row * plain;
+      tables[row * a.pstride + head_table_at<V, IL, FULL>(p, false, nslots, a.hd)] = 1.f;
+      tables[row * a.pstride + head_table_at<V, IL, FULL>(p, true, nslots, a.hd)] = 0.f;
     }
     if constexpr (BWD && NORM != 0) {
       for (int i = tid; i < 2 * NV * 16 * BLOCK; i += BLOCK) sums[i] = 0.f;
@@ -683,12 +685,12 @@ __global__ void __launch_bounds__(head_block(R), head_ctas(BWD, R, NORM, PAD)) h
       const int vec = o / (16 * tph), rest = o - vec * 16 * tph;
       const int el = rest / tph, ln = rest - el * tph;
       const int s = ln + el / (2 * V) * tph, half = el / V % 2;
-      const bool in = (!IL && s * V < pairs) || 2 * s + half < vectors;
+      const bool in = FULL != 0 ? 2 * s < vectors : (!IL && s * V < pairs) || 2 * s + half < vectors;
       if (!in) continue;
       float t = 0.f;
       for (int gr = 0; gr < groups; ++gr)
         t += sums[(vec * 16 + el / CW * CW) * BLOCK + (gr * tph + ln) * CW + el % CW];
-      w[vec * a.hd + head_col<V, IL>(s, half, pairs) + el % V] = t;
+      w[vec * a.hd + head_col<V, IL, FULL>(s, half, pairs, a.hd) + el % V] = t;
     }
   }
 }
