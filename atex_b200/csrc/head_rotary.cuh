@@ -331,18 +331,19 @@ __global__ void __launch_bounds__(head_block(R), head_ctas(BWD, R, NORM, PAD)) h
     const HeadPart& hp = a.part[part];
     const int u = i + ((first - (part ? a.q_steps : 0)) << glog);
     const int lt = static_cast<int>(fast_div(static_cast<unsigned>(u), hp.div));
+    const int h = u - lt * hp.heads;
     src = {nullptr, nullptr};
     dst = {nullptr, 0, 0};
     if (lt < tokens) {
-      const int64_t h = u - lt * hp.heads;
       const unsigned n = n0 + lt, b = fast_div(n, a.tdiv);
       const int64_t t = n - b * static_cast<unsigned>(a.T);
-      src.x = static_cast<const T*>(hp.x) + (b * hp.xs[0] + t * hp.xs[1] + h * hp.xs[2]);
-      if constexpr (BWD) src.dy = static_cast<const T*>(hp.dy) + (b * hp.ds[0] + t * hp.ds[1] + h * hp.ds[2]);
-      dst.out = static_cast<T*>(hp.out) + (b * hp.os[0] + t * hp.os[1] + h * hp.os[2]);
+      src.x = static_cast<const T*>(hp.x) + (b * hp.xs[0] + t * hp.xs[1] + static_cast<int64_t>(h) * hp.xs[2]);
+      if constexpr (BWD) src.dy = static_cast<const T*>(hp.dy) + (b * hp.ds[0] + t * hp.ds[1] + static_cast<int64_t>(h) * hp.ds[2]);
+      dst.out = static_cast<T*>(hp.out) + (b * hp.os[0] + t * hp.os[1] + static_cast<int64_t>(h) * hp.os[2]);
       dst.angles = lt * a.pstride;
     }
   };
+  const int a_row = static_cast<int>(fast_div(tid, a.adiv));   // of the angle table
   auto tokens_of = [&](int64_t block) {
     const int64_t left = a.N - block * a.tile;
     return static_cast<int>(left < a.tile ? left : a.tile);
@@ -363,22 +364,26 @@ __global__ void __launch_bounds__(head_block(R), head_ctas(BWD, R, NORM, PAD)) h
       sources[buf * a.rows + i] = src;
       targets[buf * a.rows + i] = dst;
     }
-    for (int i = tid; i < tokens * pairs; i += BLOCK) {
-      const int lt = static_cast<int>(fast_div(static_cast<unsigned>(i), a.pdiv)), p = i - lt * pairs;
-      const unsigned n = n0 + lt, b = fast_div(n, a.tdiv);
-      const int64_t t = n - b * static_cast<unsigned>(a.T);
+    // a thread keeps its pair over several tokens
+    for (int p = tid - a_row * a.across; a_row < a.down && p < pairs; p += a.across) {
       const int axis = __ldg(a.pair_axis + p);
-      float c = 1.f, s = 0.f;
-      if (axis >= 0 && axis < a.axes) {
-        const int64_t at = axis * a.ps[0] + b * a.ps[1] + t * a.ps[2];
-        const double pos = a.pos64 ? static_cast<double>(__ldg(static_cast<const long long*>(a.positions) + at))
-                                   : static_cast<double>(__ldg(static_cast<const int*>(a.positions) + at));
-        double turns = pos * __ldg(a.inv_freq + p) * 0.15915494309189533577;   // 1 / (2 pi)
-        turns -= rint(turns);
-        sincospif(2.f * static_cast<float>(turns), &s, &c);
+      const bool turns_p = axis >= 0 && axis < a.axes;
+      const double freq = __ldg(a.inv_freq + p) * 0.15915494309189533577;   // 1 / (2 pi): in turns
+      float* const cos_p = tab + head_table_at<V, IL, FULL>(p, false, nslots, a.hd);
+      float* const sin_p = tab + head_table_at<V, IL, FULL>(p, true, nslots, a.hd);
+      for (int lt = a_row; lt < tokens; lt += a.down) {
+        float c = 1.f, s = 0.f;
+        if (turns_p) {
+          const unsigned n = n0 + lt, b = fast_div(n, a.tdiv);
+          const int64_t at = axis * a.ps[0] + b * a.ps[1] + static_cast<int64_t>(n - b * static_cast<unsigned>(a.T)) * a.ps[2];
+          const double pos = a.pos64 ? static_cast<double>(__ldg(static_cast<const long long*>(a.positions) + at))
+                                     : static_cast<double>(__ldg(static_cast<const int*>(a.positions) + at));
+          const double turns = pos * freq;
+          sincospif(2.f * static_cast<float>(turns - rint(turns)), &s, &c);
+        }
+        cos_p[lt * a.pstride] = c;
+        sin_p[lt * a.pstride] = s;
       }
-      tab[lt * a.pstride + head_table_at<V, IL, FULL>(p, false, nslots, a.hd)] = c;
-      tab[lt * a.pstride + head_table_at<V, IL, FULL>(p, true, nslots, a.hd)] = s;
     }
   };
 

@@ -102,7 +102,6 @@ int fill(const nvn_head_problem& p, const nvn_heads* const (&out)[2], const nvn_
   a->N = p.batch * p.tokens;
   a->T = p.tokens;
   a->tdiv = head_divider(p.tokens);
-  a->pdiv = head_divider(p.pairs);
   a->hd = static_cast<int>(p.head_dim);
   a->inv_hd = 1.0f / static_cast<float>(p.head_dim);
   a->eps = p.epsilon;

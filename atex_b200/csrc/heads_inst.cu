@@ -27,7 +27,7 @@ namespace nvn {
 namespace {
 
 constexpr bool kBwd = NVN_BWD != 0;
-constexpr int kMaxRows = 256;            // of a tile (its addresses: 3 buffers of 32 bytes a row)
+constexpr int kMaxRows = kBwd ? 256 : 512;   // of a tile (its addresses: 3 buffers of 32 bytes a row)
 constexpr int kTableBytes = 48 * 1024;   // most that a tile's angles may take
 
 inline int round4(int v) { return (v + 3) / 4 * 4; }
@@ -42,7 +42,11 @@ cudaError_t launch_kernel(HeadArgs a, cudaStream_t s, bool dry_run, HeadPlan* pl
   a.tph = 1;
   while (a.tph * SPT < slots) a.tph *= 2;
   if (a.tph > 32) return cudaErrorInvalidValue;
-  a.pstride = a.tph * SPT * V * 2;
+  // (four lanes a head: rows of two tokens meet in one access to the table and must not share banks)
+  a.pstride = a.tph * SPT * V * 2 + (a.tph == 4 ? 16 : 0);
+  a.across = a.pairs < BLOCK ? (a.pairs > 0 ? a.pairs : 1) : BLOCK;
+  a.down = BLOCK / a.across;
+  a.adiv = head_divider(a.across);
   a.hd4 = round4(a.hd);
   // A tile is up to eight steps of the CTA.  Tokens are dealt out so that the CTAs that fit on the
   // GPU at once take the same number of tiles; when there are fewer tokens than CTAs a tile is a
@@ -70,7 +74,10 @@ cudaError_t launch_kernel(HeadArgs a, cudaStream_t s, bool dry_run, HeadPlan* pl
   int64_t room = (227 * 1024) / head_ctas(kBwd, R, NORM, PAD) - 1024 - static_cast<int64_t>(fixed) -
                  3 * 32 * (most_steps + 2) * groups;
   if (room > kTableBytes) room = kTableBytes;
-  if (tile > room / (3 * 4 * a.pstride)) tile = room / (3 * 4 * a.pstride);
+  // (unless that leaves too few rows to fill the steps: a CTA less is the smaller loss)
+  const int64_t fits = room / (3 * 4 * a.pstride);
+  if (tile > fits && fits * (hq + hk) >= 3 * groups) tile = fits;
+  if (tile > kTableBytes / (3 * 4 * a.pstride)) tile = kTableBytes / (3 * 4 * a.pstride);
   if (tile < 1) tile = 1;
   const int64_t waves = (a.N + tile * ctas - 1) / (tile * ctas);
   tile = (a.N + waves * ctas - 1) / (waves * ctas);

@@ -381,7 +381,9 @@ struct HeadArgs {
   int64_t ps[3];          // strides of positions: axis, batch, token
   int pos64, axes, pairs;
   int64_t N, T, tiles;    // N = batch * tokens
-  HeadDiv tdiv, pdiv;     // by T, by pairs
+  HeadDiv tdiv;           // by T
+  HeadDiv adiv;           // by across
+  int across, down;       // the angle table is made by `down` tokens of `across` pairs at a time
   int hd, hd4, tph, pstride;
   int tile;               // tokens of a block
   int q_steps, all_steps; // steps of a block: one row for every group of lanes each, queries first

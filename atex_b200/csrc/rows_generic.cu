@@ -239,7 +239,16 @@ __global__ void __launch_bounds__(kSumX* TY)
   griddep_wait();  // the partial rows come from the kernel launched just before
   float s = 0.f;
   if (col < cols) {
-    for (int64_t p = ty; p < rows; p += TY) s += partials[p * cols + col];
+    constexpr int U = 8;   // loads in flight; the additions keep their order
+    int64_t p = ty;
+    for (; p + (U - 1) * TY < rows; p += U * TY) {
+      float v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] = partials[(p + u * TY) * cols + col];
+#pragma unroll
+      for (int u = 0; u < U; ++u) s += v[u];
+    }
+    for (; p < rows; p += TY) s += partials[p * cols + col];
   }
   tile[ty][tx] = s;
   __syncthreads();
