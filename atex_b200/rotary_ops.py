@@ -159,6 +159,11 @@ class _Form:
         self.pos = pos
         self.q = _layout(q)
         self.k = (0, 0, 0, 0) if k is None else _layout(k)
+        self.device, self.index = q.device, q.get_device()
+        # contiguous tensors of q's and k's shape: fresh outputs, and most gradients
+        self.q_shape, self.k_shape = q.shape, None if k is None else k.shape
+        self.q_packed = (H, T * H * D, H * D, D)
+        self.k_packed = None if k is None else (kh, T * kh * D, kh * D, D)
         self.workspace = None
 
     def workspace_bytes(self, index):
@@ -182,7 +187,7 @@ def _layout(t):
 
 
 def _key(t):
-    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+    return t if t is None else (t.shape, t.stride(), t.dtype, t.device)
 
 
 # A call's checks depend on shapes, types, strides, devices and options alone, and a decoding step
@@ -225,14 +230,30 @@ def _pack(t):
     return None if t is None else _HEADS.pack(t.data_ptr(), *_layout(t))
 
 
-def _outputs(q, k, out):
+def _outputs(form, q, k, out):
+    """The two outputs and their nvn_heads."""
     if out is None:
-        return q.new_empty(q.shape), None if k is None else k.new_empty(k.shape)
+        q_out = q.new_empty(form.q_shape)
+        if k is None:
+            return q_out, None, _HEADS.pack(q_out.data_ptr(), *form.q_packed), None
+        k_out = k.new_empty(form.k_shape)
+        return (q_out, k_out, _HEADS.pack(q_out.data_ptr(), *form.q_packed),
+                _HEADS.pack(k_out.data_ptr(), *form.k_packed))
     q_out, k_out = out
     _checked_out(q_out, q, "out[0]")
-    if k is not None:
-        _checked_out(k_out, k, "out[1]")
-    return q_out, k_out
+    if k is None:
+        return q_out, None, _pack(q_out), None
+    _checked_out(k_out, k, "out[1]")
+    return q_out, k_out, _pack(q_out), _pack(k_out)
+
+
+def _gradient(g, shape, dtype, form, name):
+    """A gradient as the kernels can read it."""
+    if not isinstance(g, torch.Tensor) or g.shape != shape or g.dtype != dtype:
+        raise InvalidArgumentError(f"{name} must have the shape and dtype of its input")
+    if g.device != form.device:
+        _on_cuda(g, name, form.device)
+    return _rows_contiguous(g)
 
 
 def fused_head_norm_rotary_op(q, k, positions, inv_freq=None, pair_axis=None, scale_q=None, scale_k=None,
@@ -248,10 +269,10 @@ def fused_head_norm_rotary_op(q, k, positions, inv_freq=None, pair_axis=None, sc
     themselves."""
     form, packed, q, k, alive = _problem(q, k, positions, inv_freq, pair_axis, (scale_q, scale_k),
                                          (offset_q, offset_k), norm, interleaved, epsilon, True)
-    q_out, k_out = _outputs(q, k, out)
+    q_out, k_out, to_q, to_k = _outputs(form, q, k, out)
     if form.empty:
         return q_out, k_out
-    st = _on_stream(q.get_device(), _lib.load().nvn_head_norm_rotary_fwd, packed, _pack(q_out), _pack(k_out))
+    st = _on_stream(form.index, _lib.load().nvn_head_norm_rotary_fwd, packed, to_q, to_k)
     _check(st, "nvn_head_norm_rotary_fwd")
     return q_out, k_out
 
@@ -266,26 +287,21 @@ def fused_head_norm_rotary_grad_op(q_backprop, k_backprop, q, k, positions, inv_
     form, packed, q, k, alive = _problem(q, k, positions, inv_freq, pair_axis, (scale_q, scale_k), (None, None), norm,
                                          interleaved, epsilon, False)
     _require((k is None) == (k_backprop is None), "k_backprop belongs to k")
-    grads = [None, None]
-    for i, (g, x, name) in enumerate(((q_backprop, q, "q_backprop"), (k_backprop, k, "k_backprop"))):
-        if x is not None:
-            if not isinstance(g, torch.Tensor) or g.shape != x.shape or g.dtype != x.dtype:
-                raise InvalidArgumentError(f"{name} must have the shape and dtype of its input")
-            _on_cuda(g, name, x.device)
-            grads[i] = _rows_contiguous(g)
-    dq, dk = _outputs(q, k, out)
+    q_backprop = _gradient(q_backprop, form.q_shape, q.dtype, form, "q_backprop")
+    if k is not None:
+        k_backprop = _gradient(k_backprop, form.k_shape, q.dtype, form, "k_backprop")
+    dq, dk, to_q, to_k = _outputs(form, q, k, out)
     dparams = ws = None
     if form.vectors:
         dparams = scale_q.new_empty((form.parts * form.vectors, form.head_dim))
         if form.empty:
             dparams.zero_()
     if not form.empty:
-        index = q.get_device()
-        nbytes = form.workspace_bytes(index)
+        nbytes = form.workspace_bytes(form.index)
         if nbytes:
             ws = _scratch(scale_q, nbytes)
-        st = _on_stream(index, _lib.load().nvn_head_norm_rotary_bwd, packed, _pack(grads[0]), _pack(grads[1]),
-                        _pack(dq), _pack(dk), _ptr(dparams), _ptr(ws), nbytes)
+        st = _on_stream(form.index, _lib.load().nvn_head_norm_rotary_bwd, packed, _pack(q_backprop),
+                        _pack(k_backprop), to_q, to_k, _ptr(dparams), _ptr(ws), nbytes)
         _check(st, "nvn_head_norm_rotary_bwd")
     if dparams is None:
         return dq, dk, None, None, None, None
