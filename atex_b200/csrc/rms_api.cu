@@ -182,7 +182,8 @@ int nvn_rms_fwd_residual(int dtype, const void* x, const void* residual, const f
                          float* inv_rms, void* stream) {
   if (!valid_dtype(dtype) || N < 0 || D < 0) return NVN_ERR_INVALID_ARGUMENT;
   if (N == 0 || D == 0) return NVN_OK;
-  if (x == nullptr || residual == nullptr || gamma == nullptr || sum_out == nullptr || y == nullptr)
+  if (x == nullptr || residual == nullptr || gamma == nullptr || sum_out == nullptr || y == nullptr ||
+      sum_out == y)
     return NVN_ERR_INVALID_ARGUMENT;
   return forward(dtype, x, residual, gamma, N, D, epsilon, sum_out, y, inv_rms,
                  static_cast<cudaStream_t>(stream));

@@ -155,7 +155,7 @@ class _Form:
         self.copies = self.copies or any(t is not None and _rows_contiguous(t) is not t for t in (q, k))
         self.empty = B * T == 0
         position_bytes = 8 if positions is None or positions.dtype == torch.int64 else 4
-        self.head = (code, norm_code, int(bool(interleaved)), float(epsilon), B, T, D, pairs, axes, position_bytes)
+        self.head = (code, norm_code, int(interleaved), epsilon, B, T, D, pairs, axes, position_bytes)
         self.pos = pos
         self.q = _layout(q)
         self.k = (0, 0, 0, 0) if k is None else _layout(k)
@@ -197,6 +197,7 @@ _forms = {}
 
 def _problem(q, k, positions, inv_freq, pair_axis, scales, offsets, norm, interleaved, epsilon, want_offsets):
     """The checked form of a call, its nvn_head_problem, and q and k as the kernels can read them."""
+    interleaved, epsilon = bool(interleaved), float(epsilon)
     try:
         key = (_key(q), _key(k), _key(positions), _key(inv_freq), _key(pair_axis), _key(scales[0]), _key(scales[1]),
                _key(offsets[0]), _key(offsets[1]), norm, interleaved, epsilon, want_offsets)
@@ -318,6 +319,7 @@ class _head_norm_rotary_grad(torch.autograd.Function):
                                         **form)
         ctx.save_for_backward(q, k, scale_q, scale_k, positions, inv_freq, pair_axis)
         ctx.form = form
+        ctx.shapes = [None if t is None else t.shape for t in (scale_q, scale_k, offset_q, offset_k)]
         ctx.set_materialize_grads(False)
         return out
 
@@ -330,9 +332,8 @@ class _head_norm_rotary_grad(torch.autograd.Function):
             grad_k = torch.zeros_like(k)
         dq, dk, gq, gk, oq, ok = fused_head_norm_rotary_grad_op(grad_q, grad_k, q, k, positions, inv_freq, pair_axis,
                                                                 scale_q, scale_k, **ctx.form)
-        like = [None if g is None or s is None else g.view(s.shape)
-                for g, s in ((gq, scale_q), (gk, scale_k), (oq, scale_q), (ok, scale_k))]
-        return dq, dk, *like, None, None, None, None
+        sums = [None if g is None else g.view(s) for g, s in zip((gq, gk, oq, ok), ctx.shapes)]
+        return dq, dk, *sums, None, None, None, None
 
 
 def head_norm_rotary(q, k, positions, inv_freq=None, pair_axis=None, scale_q=None, scale_k=None, offset_q=None,

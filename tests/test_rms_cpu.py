@@ -60,11 +60,12 @@ def test_abi_refuses_before_it_touches_cuda(lib):
     assert lib.nvn_rms_fwd(0, n, n, 0, 4, 1e-3, n, n, n) == L.NVN_OK
     assert lib.nvn_rms_fwd_residual(0, n, n, n, 4, 4, 1e-3, n, n, n, n) == bad
     assert lib.nvn_rms_fwd_residual(2, n, n, n, 4, 0, 1e-3, n, n, n, n) == L.NVN_OK
+    buf = (ctypes.c_float * 64)()
+    p = ctypes.cast(buf, ctypes.c_void_p)
+    assert lib.nvn_rms_fwd_residual(0, p, p, p, 4, 4, 1e-3, p, p, n, n) == bad      # one place for two outputs
     assert lib.nvn_rms_bwd(0, n, n, n, n, n, 4, 4, n, n, n, 0, n) == bad
     assert lib.nvn_rms_bwd(0, n, n, n, n, n, 4, 0, n, n, n, 0, n) == L.NVN_OK
     assert lib.nvn_ln_bwd_residual(0, n, n, n, n, n, n, 4, 4, n, n, n, n, 0, n) == bad
-    buf = (ctypes.c_float * 64)()
-    p = ctypes.cast(buf, ctypes.c_void_p)
     off = ctypes.c_void_p((p.value + 255) // 256 * 256 + 4)
     # a workspace that is missing or misaligned is an error and not a write
     for ws in (n, off):

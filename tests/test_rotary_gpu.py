@@ -294,6 +294,18 @@ def test_values_at_the_edges(lib):
         c["q"][0, 1, 1, 100] = float("inf")
         q, _ = forward(c)
         assert torch.isinf(q[0, 1, 1, 100]) and int(torch.isfinite(q).logical_not().sum()) == 1
+    # nor where the rotated elements end inside a vector
+    for hd, pairs, at in ((72, 11, 22), (72, 11, 23), (64, 5, 10), (100, 3, 7)):
+        c = case(1, 8, 4, 2, hd, pairs, "none", True, "bf16", 9)
+        c["q"][0, 1, 1, at] = float("inf")
+        q, _ = forward(c)
+        assert torch.isinf(q[0, 1, 1, at]) and int(torch.isfinite(q).logical_not().sum()) == 1
+    # a gradient's infinity reaches its own head's row and columns, and nothing of a step's empty rows
+    c = case(1, 3, 3, 1, 128, 64, "layer", False, "bf16", 11)
+    c["dq"][0, 0, 0, 0] = float("inf")
+    dq, dk, gq, gk, oq, ok = backward(c)
+    assert torch.isfinite(dq[0, 1:]).all() and torch.isfinite(dq[0, 0, 1:]).all() and torch.isfinite(dk).all()
+    assert all(torch.isfinite(t).all() for t in (gk, ok, gq[1:64], gq[65:], oq[1:64], oq[65:]))
     # every token's row of zeros without epsilon: nothing from it reaches the parameter sums of the others
     c = case(1, 9, 1, 1, 96, 48, "rms", False, "f32", 10)
     check_both(c)
@@ -427,6 +439,44 @@ def test_gradients_against_differences(lib, norm):
             terms = grad.double() * v
             # h^2 times a third derivative, and fp32 sums of a few thousand terms: far below 1e-5 of sum|terms|
             assert abs(float(terms.sum() - diff)) <= 1e-5 * float(terms.abs().sum())
+
+
+def test_a_captured_training_step(lib):
+    """Forward and backward through autograd in one captured graph, replayed on new values."""
+    B, T_, hq, hk, hd = 2, 40, 4, 2, 64
+    c = case(B, T_, hq, hk, hd, 32, "rms", False, "bf16", 61)
+    x = torch.randn(B, T_, (hq + 2 * hk) * hd, device=DEV).bfloat16()
+    up = torch.randn(B, T_, hq, hd, device=DEV).bfloat16()
+
+    def step(leaf, sq, sk):
+        qkv = leaf.view(B, T_, hq + 2 * hk, hd)
+        q, k = A.head_norm_rotary(qkv[:, :, :hq], qkv[:, :, hq:hq + hk], c["positions"], c["freq"], c["axis"], sq, sk,
+                                  epsilon=EPS)
+        torch.autograd.backward([q, k], [up, up[:, :, :hk]])
+
+    def leaves():
+        return x.clone().requires_grad_(), c["scale_q"].clone().requires_grad_(), c["scale_k"].clone().requires_grad_()
+    static = leaves()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(*static)
+    torch.cuda.current_stream().wait_stream(side)
+    for t in static:
+        t.grad = None
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step(*static)
+    x = torch.randn_like(x)
+    with torch.no_grad():
+        static[0].copy_(x)
+    g.replay()
+    torch.cuda.synchronize()
+    eager = leaves()
+    step(*eager)
+    for a, b in zip(static, eager):
+        assert torch.equal(a.grad, b.grad)
 
 
 def test_refusals_that_need_a_device(lib):
