@@ -149,8 +149,7 @@ size_t nvn_head_norm_rotary_bwd_workspace_bytes(const nvn_head_problem* p) {
       (void)cudaGetLastError();
       return 0;
     }
-    const size_t b = static_cast<size_t>(plan.grid) * a.parts * vectors_per_part(p->norm) * a.hd * 4;
-    if (b > most) most = b;
+    if (plan.ws_bytes > most) most = plan.ws_bytes;
   }
   return align_up(most, 256);
 }
@@ -177,11 +176,11 @@ int nvn_head_norm_rotary_bwd(const nvn_head_problem* p, const nvn_heads* q_grad,
   HeadArgs a;
   const int v = fill(*p, {dq, k ? dk : nullptr}, {q_grad, k ? k_grad : nullptr}, &a);
   a.ws = static_cast<float*>(workspace);
+  a.ws_bytes = workspace_bytes;
   HeadPlan plan;
-  cudaError_t e = heads_fn(p->dtype, true)(p->norm, p->interleaved != 0, v, a, s, true, &plan);
+  cudaError_t e = heads_fn(p->dtype, true)(p->norm, p->interleaved != 0, v, a, s, false, &plan);
   if (e != cudaSuccess) return fail_cuda(e);
-  if (workspace_bytes < static_cast<size_t>(plan.grid) * cols * 4) return NVN_ERR_WORKSPACE;
-  e = heads_fn(p->dtype, true)(p->norm, p->interleaved != 0, v, a, s, false, &plan);
+  if (plan.ws_bytes > workspace_bytes) return NVN_ERR_WORKSPACE;
   if (e == cudaSuccess && cols > 0) e = colsum_launch(a.ws, plan.grid, cols, dparams, s);
   return e == cudaSuccess ? NVN_OK : fail_cuda(e);
 }

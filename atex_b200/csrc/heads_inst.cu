@@ -115,7 +115,8 @@ cudaError_t launch_kernel(HeadArgs a, cudaStream_t s, bool dry_run, HeadPlan* pl
   plan->v = V;
   plan->grid = static_cast<int>(grid);
   plan->smem = smem;
-  if (dry_run) return cudaSuccess;
+  plan->ws_bytes = kBwd ? static_cast<size_t>(grid) * a.parts * NV * a.hd * 4 : 0;
+  if (dry_run || plan->ws_bytes > a.ws_bytes) return cudaSuccess;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
   cfg.blockDim = dim3(BLOCK, 1, 1);

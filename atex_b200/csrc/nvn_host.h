@@ -375,6 +375,7 @@ struct HeadArgs {
   int parts;
   const float* param[4];  // scale and offset of the queries, scale and offset of the keys
   float* ws;              // partial rows [grid][parts][1 or 2][hd]
+  size_t ws_bytes;
   const void* positions;
   const double* inv_freq;
   const int32_t* pair_axis;
@@ -395,6 +396,7 @@ struct HeadPlan {
   int v;                  // elements per access
   int grid;               // CTAs = partial rows
   size_t smem;
+  size_t ws_bytes;        // of the partial rows; nothing is launched when HeadArgs has fewer
 };
 // `bwd`, `norm` (0 none, 1 root mean square, 2 mean and variance), `interleaved` select the
 // kernel; the launcher sets the layout (hd4, tph, pstride, tile ... rows, tiles) itself.  With dry_run nothing is launched.

@@ -231,13 +231,18 @@ def _pack(t):
     return None if t is None else _HEADS.pack(t.data_ptr(), *_layout(t))
 
 
+def _fresh(like):
+    """A contiguous tensor like `like` (empty_like is the cheaper call, but keeps a view's strides)."""
+    return torch.empty_like(like) if like.is_contiguous() else like.new_empty(like.shape)
+
+
 def _outputs(form, q, k, out):
-    """The two outputs and their nvn_heads."""
+    """The two outputs, of the shapes of q and k or their gradients, and their nvn_heads."""
     if out is None:
-        q_out = q.new_empty(form.q_shape)
+        q_out = _fresh(q)
         if k is None:
             return q_out, None, _HEADS.pack(q_out.data_ptr(), *form.q_packed), None
-        k_out = k.new_empty(form.k_shape)
+        k_out = _fresh(k)
         return (q_out, k_out, _HEADS.pack(q_out.data_ptr(), *form.q_packed),
                 _HEADS.pack(k_out.data_ptr(), *form.k_packed))
     q_out, k_out = out
@@ -291,7 +296,7 @@ def fused_head_norm_rotary_grad_op(q_backprop, k_backprop, q, k, positions, inv_
     q_backprop = _gradient(q_backprop, form.q_shape, q.dtype, form, "q_backprop")
     if k is not None:
         k_backprop = _gradient(k_backprop, form.k_shape, q.dtype, form, "k_backprop")
-    dq, dk, to_q, to_k = _outputs(form, q, k, out)
+    dq, dk, to_q, to_k = _outputs(form, q_backprop, k_backprop, out)
     dparams = ws = None
     if form.vectors:
         dparams = scale_q.new_empty((form.parts * form.vectors, form.head_dim))

@@ -328,6 +328,26 @@ def test_offsets_beyond_32_bits(lib):
     assert torch.equal(far, want[0])
 
 
+def test_workspace_too_small_is_an_error_and_not_a_write(lib):
+    from atex_b200 import rotary_ops as R
+    c = case(2, 300, 4, 2, 64, 32, "layer", False, "bf16", 1)
+    form, packed, q, k, alive = R._problem(c["q"], c["k"], c["positions"], c["freq"], c["axis"],
+                                           (c["scale_q"], c["scale_k"]), (None, None), "layer", False, EPS, False)
+    need = lib.nvn_head_norm_rotary_bwd_workspace_bytes(packed)
+    assert need == form.workspace_bytes(0) and need >= 4 * 64 * 4
+    ws = torch.full((need // 4,), 7.0, device=DEV)
+    out = torch.full((2, 2, 64), 7.0, device=DEV)
+    dq, dk = torch.full_like(q, 7.0), torch.full_like(k, 7.0)
+    args = (packed, R._pack(c["dq"]), R._pack(c["dk"]), R._pack(dq), R._pack(dk), out.data_ptr(), ws.data_ptr())
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.nvn_head_norm_rotary_bwd(*args, 256, stream) == _lib.NVN_ERR_WORKSPACE
+    torch.cuda.synchronize()
+    assert all((t == 7).all() for t in (ws, out, dq, dk))
+    assert lib.nvn_head_norm_rotary_bwd(*args, need, stream) == _lib.NVN_OK
+    want = backward(c)
+    assert torch.equal(dq, want[0]) and torch.equal(dk, want[1]) and torch.equal(out[0, 0], want[2])
+
+
 def test_empty_batches(lib):
     for B, T_ in ((0, 5), (3, 0)):
         c = case(B, T_, 4, 2, 64, 32, "layer", False, "bf16", 1)
