@@ -294,9 +294,11 @@ cudaError_t residual_add_launch(int dtype, const void* x, const void* res, void*
 //     one reduction does not hide (bf16 [32768, 4096] plain 97 -> 84 us, residual 181 -> 164 us,
 //     where 192 threads of which 21 idle at the end beat 128 that fit); wide rows of the residual
 //     form load on demand ([16384, 8192] 186 -> 166 us, [4096, 32768] 219 -> 177 us).
-//   backward: two stages and a warp or two per row (f16 [65536, 1024] 93 -> 85 us LayerNorm,
-//     bf16 [32768, 2048] 107 -> 84 us RMS residual); with the dbeta sums 128 threads a row keep
-//     164 us at [32768, 4096] where 256 take 187, without them 256 win (141 -> 126 us).
+//   backward: two stages and a warp or two per row (f16 [65536, 1024] LayerNorm 93 -> 85 us, bf16
+//     [32768, 2048] RMS residual 107 -> 84 us).  Where three tensors are read, two rows at once and
+//     CTAs of 256 threads, whose half as many partial rows cost less to write and read, win again
+//     (bf16 [32768, 4096] RMS residual 169 -> 159 us, LayerNorm 161 us); with two tensors one row
+//     does (134 -> 125 us).
 constexpr int64_t kRmsHeldMinBytes = 32ll << 20;
 #define NVN_RMS_FWD_SHAPES(X)                                                                  \
   X(0, 4, 1, 4, 128, 1, 3)    X(1, 8, 1, 4, 128, 1, 3)    X(2, 8, 2, 4, 128, 1, 3)              \
@@ -307,17 +309,18 @@ constexpr int64_t kRmsHeldMinBytes = 32ll << 20;
   X(15, 512, 2, 1, 0, 1, 1)   X(16, 256, 4, 1, 0, 0, 2)   X(17, 320, 4, 1, 0, 1, 1)             \
   X(18, 320, 4, 1, 0, 0, 2)   X(19, 384, 4, 1, 0, 1, 1)   X(20, 384, 4, 1, 0, 0, 2)             \
   X(21, 512, 4, 1, 0, 1, 3)   X(22, 512, 8, 1, 0, 0, 3)
-#define NVN_RMS_BWD_SHAPES(X)                                                                  \
-  X(0, 4, 1, 4, 128, 1, 7)    X(1, 8, 1, 4, 128, 1, 7)    X(2, 8, 2, 4, 128, 12, 7)             \
-  X(3, 16, 1, 4, 128, 1, 7)   X(4, 16, 2, 4, 128, 12, 7)  X(5, 32, 1, 4, 128, 1, 7)             \
-  X(6, 32, 2, 4, 128, 12, 7)  X(7, 32, 2, 2, 128, 1, 7)   X(8, 32, 3, 2, 128, 12, 7)            \
-  X(9, 32, 3, 1, 128, 1, 7)   X(10, 32, 4, 2, 128, 12, 7) X(11, 32, 4, 1, 128, 1, 7)            \
-  X(12, 64, 3, 2, 128, 12, 7) X(13, 64, 3, 1, 128, 1, 7)  X(14, 64, 4, 2, 128, 12, 7)           \
-  X(15, 128, 2, 1, 128, 1, 7) X(16, 128, 3, 1, 128, 12, 7) X(17, 128, 3, 1, 128, 1, 7)          \
-  X(18, 256, 2, 1, 0, 12, 3)  X(19, 256, 2, 1, 0, 1, 3)   X(20, 128, 4, 1, 128, 12, 4)          \
-  X(21, 128, 4, 1, 128, 1, 4) X(22, 128, 5, 1, 128, 12, 7) X(23, 320, 2, 1, 0, 1, 7)            \
-  X(24, 256, 3, 1, 0, 12, 7)  X(25, 256, 3, 1, 0, 1, 7)   X(26, 256, 4, 1, 0, 12, 7)            \
-  X(27, 512, 2, 1, 0, 1, 7)   X(28, 512, 3, 1, 0, 12, 7)  X(29, 512, 4, 1, 0, 12, 7)
+#define NVN_RMS_BWD_SHAPES(X)                                                                 \
+  X(0, 4, 1, 4, 128, 1, 7)      X(1, 8, 1, 4, 128, 1, 7)      X(2, 8, 2, 4, 128, 12, 7)       \
+  X(3, 16, 1, 4, 128, 1, 7)     X(4, 16, 2, 4, 128, 12, 7)    X(5, 32, 1, 4, 128, 1, 7)       \
+  X(6, 32, 2, 4, 128, 12, 7)    X(7, 32, 2, 2, 128, 1, 7)     X(8, 32, 3, 2, 128, 12, 7)      \
+  X(9, 32, 3, 1, 128, 1, 7)     X(10, 32, 4, 2, 128, 12, 1)   X(11, 64, 2, 2, 0, 12, 6)       \
+  X(12, 32, 4, 1, 128, 1, 7)    X(13, 64, 3, 2, 128, 12, 7)   X(14, 64, 3, 1, 128, 1, 7)      \
+  X(15, 64, 4, 2, 128, 12, 3)   X(16, 64, 4, 2, 0, 12, 4)     X(17, 128, 2, 1, 128, 1, 7)     \
+  X(18, 128, 3, 1, 128, 12, 7)  X(19, 128, 3, 1, 128, 1, 7)   X(20, 256, 2, 1, 0, 12, 1)      \
+  X(21, 256, 2, 2, 0, 12, 6)    X(22, 256, 2, 1, 0, 1, 3)     X(23, 128, 4, 1, 128, 1, 4)     \
+  X(24, 128, 5, 1, 128, 12, 7)  X(25, 320, 2, 1, 0, 1, 7)     X(26, 256, 3, 1, 0, 12, 7)      \
+  X(27, 256, 3, 1, 0, 1, 7)     X(28, 256, 4, 1, 0, 12, 7)    X(29, 512, 2, 1, 0, 1, 7)       \
+  X(30, 512, 3, 1, 0, 12, 7)    X(31, 512, 4, 1, 0, 12, 7)
 // Accesses of less than 128 bits.  Against the LayerNorm table: f16 [12345, 1001] 20.3 -> 12.5 us
 // forward, 58 -> 34 us LayerNorm backward; bf16 [29363, 2347] residual 258 -> 122 us.  The widest
 // entry holds 16 values of four tensors per thread, too many with the dbeta sums (f16 [4000, 7031]
