@@ -40,13 +40,13 @@
 namespace nvn {
 
 // Threads per CTA, and the CTAs per SM that the registers are limited for: with two rows at once
-// 5, with offsets 4, (backward 4, with offsets or padding 3) small CTAs of up to 102, 128 (128,
-// 168) registers; with one row 3 (2) of 80 (128).  Spilling to fit a fourth cost more than it gave (88 -> 115 us).  Small
+// 5 (backward 4) small CTAs of up to 102 (128) registers, with offsets or padding one fewer of 128
+// (168); with one row 3 (2) of 80 (128).  Spilling to fit a fourth cost more than it gave (88 -> 115 us).  Small
 // CTAs for one row were slower (f32 [3, 1025, 10+2, 80] gradient 17.5 -> 20.0 us).
 __host__ __device__ constexpr int head_block(int rows) { return rows > 1 ? 128 : 256; }
 __host__ __device__ constexpr int head_ctas(bool bwd, int rows, int norm, bool pad) {
   return bwd ? (rows > 1 ? (norm == 2 || (norm == 1 && pad) ? 3 : 4) : 2)
-             : (rows > 1 ? (norm == 2 ? 4 : 5) : 3);
+             : (rows > 1 ? (norm == 2 || pad ? 4 : 5) : 3);
 }
 
 // n / d for n < 2^31 by a multiplication: with 2^(s-1) < d <= 2^s and m = ceil(2^(31+s) / d),

@@ -42,8 +42,7 @@ cudaError_t launch_kernel(HeadArgs a, cudaStream_t s, bool dry_run, HeadPlan* pl
   a.tph = 1;
   while (a.tph * SPT < slots) a.tph *= 2;
   if (a.tph > 32) return cudaErrorInvalidValue;
-  // (four lanes a head: rows of two tokens meet in one access to the table and must not share banks)
-  a.pstride = a.tph * SPT * V * 2 + (a.tph == 4 ? 16 : 0);
+  a.pstride = a.tph * SPT * V * 2;
   a.across = a.pairs < BLOCK ? (a.pairs > 0 ? a.pairs : 1) : BLOCK;
   a.down = BLOCK / a.across;
   a.adiv = head_divider(a.across);

@@ -147,11 +147,8 @@ int backward(int form, int dtype, const void* dy, const void* dsum, const void* 
                        static_cast<int>(p.partial_rows), s);
   }
   if (e != cudaSuccess) return fail_cuda(e);
-  if (form == 2) {
-    e = colreduce_launch(a.ws, p.partial_rows, D, dgamma, dbeta, s);
-  } else {
-    e = colsum_launch(a.ws, p.partial_rows, D, dgamma, s);
-  }
+  e = form == 2 ? colreduce_launch(a.ws, p.partial_rows, D, dgamma, dbeta, s)
+                : colsum_launch(a.ws, p.partial_rows, D, dgamma, s);
   return e == cudaSuccess ? NVN_OK : fail_cuda(e);
 }
 

@@ -224,22 +224,27 @@ cudaError_t generic_t(bool vec, bool bwd, bool rms, const RowsResArgs& a, float*
 }
 
 // ---- column sum ---------------------------------------------------------------
-// Block (32, TY): thread (tx, ty) adds rows ty, ty + TY, ... of column tx in increasing order,
-// then the TY sums are added in increasing ty: a fixed order, the same bits on every run.
-constexpr int kSumX = 32;
+// Block (X, 1024 / X): thread (tx, ty) adds rows ty, ty + TY, ... of column tx in increasing order;
+// the TY sums are then added in a fixed order, so that every run gives the same bits.  The partial
+// rows come out of L2 and the kernel is a chain of its latencies: up to 2048 columns take X = 8
+// (a sector of each row), four times the CTAs and a quarter of the rows per thread of X = 32 (the
+// rotary gradients of f16 [14, 3, 32+8, 160] 8.4 -> 7.2 us and f32 [43, 23, 2+1, 128] 7.8 -> 7.3
+// us, both kernels).
+constexpr int kSumThreads = 1024;
 
-template <int TY>
-__global__ void __launch_bounds__(kSumX* TY)
+template <int X>
+__global__ void __launch_bounds__(kSumThreads)
     colsum_kernel(const float* __restrict__ partials, int64_t rows, int64_t cols,
                   float* __restrict__ out) {
-  __shared__ float tile[TY][kSumX + 1];
-  const int tx = threadIdx.x, ty = threadIdx.y;
-  const int64_t col = static_cast<int64_t>(blockIdx.x) * kSumX + tx;
+  constexpr int TY = kSumThreads / X;
+  constexpr int U = 4;   // loads in flight; the additions keep their order
+  __shared__ float tile[32][X + 1];
+  const int tid = threadIdx.x, tx = tid % X, ty = tid / X;
+  const int64_t col = static_cast<int64_t>(blockIdx.x) * X + tx;
   griddep_launch_dependents();
   griddep_wait();  // the partial rows come from the kernel launched just before
   float s = 0.f;
   if (col < cols) {
-    constexpr int U = 8;   // loads in flight; the additions keep their order
     int64_t p = ty;
     for (; p + (U - 1) * TY < rows; p += U * TY) {
       float v[U];
@@ -250,23 +255,26 @@ __global__ void __launch_bounds__(kSumX* TY)
     }
     for (; p < rows; p += TY) s += partials[p * cols + col];
   }
-  tile[ty][tx] = s;
-  __syncthreads();
-  if (ty == 0 && col < cols) {
-    float t = 0.f;
+  // the lanes of a warp that share a column, then the 32 warps
 #pragma unroll
-    for (int k = 0; k < TY; ++k) t += tile[k][tx];
-    out[col] = t;
+  for (int off = X; off < 32; off <<= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+  if (tid % 32 < X) tile[tid / 32][tx] = s;
+  __syncthreads();
+  if (tid < X && col < cols) {
+    float t[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 32; ++k) t[k % 4] += tile[k][tx];
+    out[col] = (t[0] + t[1]) + (t[2] + t[3]);
   }
 }
 
-template <int TY>
+template <int X>
 cudaError_t colsum_t(const float* partials, int64_t rows, int64_t cols, float* out, cudaStream_t s) {
   cudaLaunchAttribute attr;
   const cudaLaunchConfig_t cfg = dependent_launch_config(
-      dim3(static_cast<unsigned>((cols + kSumX - 1) / kSumX)), dim3(kSumX, TY), 0, s, &attr);
+      dim3(static_cast<unsigned>((cols + X - 1) / X)), dim3(kSumThreads), 0, s, &attr);
   count_launch();
-  return cudaLaunchKernelEx(&cfg, colsum_kernel<TY>, partials, rows, cols, out);
+  return cudaLaunchKernelEx(&cfg, colsum_kernel<X>, partials, rows, cols, out);
 }
 
 }  // namespace
@@ -288,8 +296,8 @@ cudaError_t generic_launch(int dtype, bool vec, bool bwd, bool rms, const RowsRe
 
 cudaError_t colsum_launch(const float* partials, int64_t rows, int64_t cols, float* out,
                           cudaStream_t s) {
-  return rows <= 32 ? colsum_t<4>(partials, rows, cols, out, s)
-                    : colsum_t<32>(partials, rows, cols, out, s);
+  return cols <= 2048 ? colsum_t<8>(partials, rows, cols, out, s)
+                      : colsum_t<32>(partials, rows, cols, out, s);
 }
 
 }  // namespace nvn
