@@ -128,10 +128,14 @@ def test_forward_and_gradients_over_the_widths(lib, dtype, D):
     assert lib.nvn_device_status() == _lib.NVN_OK
 
 
-# tensors of 64 MB and more take the kernels that hold a row batch in shared memory
+# tensors of 32 MB and more take the kernels that hold a row batch in shared memory
 @pytest.mark.parametrize("dtype,N,D", [("bf16", 8197, 4096), ("f16", 131, 262144), ("f32", 16401, 1024),
                                        ("bf16", 16389, 2048), ("f16", 4101, 8192), ("f32", 2053, 8192),
-                                       ("bf16", 30000, 1152), ("f16", 262147, 128)])
+                                       ("bf16", 30000, 1152), ("f16", 262147, 128), ("f16", 20003, 1024),
+                                       ("bf16", 40001, 512), ("f16", 80003, 256), ("bf16", 25001, 768),
+                                       ("bf16", 4099, 5120), ("f32", 3001, 4096), ("f16", 3001, 6144),
+                                       ("bf16", 1501, 12288), ("f32", 1101, 8000), ("bf16", 2001, 9000),
+                                       ("f16", 1501, 16384), ("f32", 12001, 768), ("bf16", 7001, 2600)])
 def test_large_tensors(lib, dtype, N, D):
     x, res, dy, ds, gamma, beta = data(N, D, dtype, N + D)
     y, s, inv = A.fused_rms_norm_residual_op(x, res, gamma, epsilon=1e-6)

@@ -187,6 +187,17 @@ def test_batches_tokens_heads_and_layouts(lib, layout, B, T_, hq, hk):
             check_both(case(B, T_, hq, hk, hd, hd // 2, norm, il, dtype, B + T_ + hq, layout=layout))
 
 
+@pytest.mark.parametrize("norm", ["none", "rms", "layer"])
+@pytest.mark.parametrize("hd,pairs", [(48, 24), (64, 32), (64, 8), (80, 40), (96, 48), (112, 56), (128, 64), (128, 16),
+                                      (160, 80), (192, 96), (192, 40), (240, 120), (256, 128), (256, 64)])
+def test_two_heads_at_once(lib, hd, pairs, norm):
+    """Even numbers of heads and enough rows: the kernels that take neighbouring heads together, with
+    lanes to spare (sizes between the powers of two) and rotated ranges that end inside the head."""
+    for dtype, il in (("bf16", False), ("f16", True)):
+        check_both(case(2, 1301, 8, 4, hd, pairs, norm, il, dtype, hd + pairs, layout="packed"))
+    check_both(case(1, 2603, 8, 4, hd, pairs, norm, True, "f32", hd + pairs))
+
+
 @pytest.mark.parametrize("axes,far,int32", [(1, 4, True), (2, 2 ** 31 - 1, True), (4, 10 ** 6, False), (1, 2 ** 40, False)])
 def test_positions(lib, axes, far, int32):
     """Far positions keep their angles: 2^40 times a frequency is still known to 1e-4 of a turn in 64
