@@ -10,7 +10,10 @@
 //   are formed again from x, whose row sits in registers anyway: one more shuffle reduction in
 //   place of two more tensors.
 //
-// Both directions are bound by HBM: 2 (forward) or 3 (gradient) passes over q and k.
+// Both directions move 2 (forward) or 3 (gradient) passes over q and k and are bound by HBM when
+// there are rows enough: bf16, 32+8 packed heads of 128, 32768 tokens forward 111 us (6.1 TB/s, 93 % of
+// the measured copy rate), 16384 tokens gradient 88 us (5.7 TB/s).  What stands between that and the
+// copy rate is a row's dependent chain (unpack, sums, shuffles, rotation) on 16 to 20 warps an SM.
 //
 // Layout.  A head is a row of head_dim elements; TPH lanes of a warp (a power of two) own it, 16
 // elements each, as SPT slots of two vectors (A, B) of V elements:
@@ -26,7 +29,7 @@
 // token are the same for all its heads and are computed once per tile into shared memory - in 64
 // bits up to the fraction of a turn, because a position of a million times a frequency has no
 // fraction left in 32.  Where each row of a tile begins is worked out once as well, by one thread a
-// row: done by every lane for every row it was two thirds of the instructions.  The rows of a tile
+// row (done by every lane for every row it was a fifth of the instructions).  The rows of a tile
 // are dealt to the groups of TPH lanes; while a group works on a row its next one is already on the
 // way into registers, across the ends of parts and tiles too.  The tables (angles, row addresses)
 // have three buffers, so that one barrier per tile is enough: tile i reads buffer i, its last rows

@@ -375,3 +375,29 @@ def test_gradients_against_differences(lib, kind):
     # values of order one are off by far less than 1e-5 of sum|terms|
     assert abs(float((dx.double() * vs).sum() - along_x)) <= 1e-5 * float((dx.double() * vs).abs().sum())
     assert abs(float((dg.double() * vg).sum() - along_g)) <= 1e-5 * float((dg.double() * vg).abs().sum())
+
+
+@pytest.mark.parametrize("dtype,N,D", [("f32", 200003, 3), ("bf16", 100001, 17), ("f16", 3, 1000003), ("bf16", 2, 500008)])
+def test_many_short_rows_and_few_long_ones(lib, dtype, N, D):
+    x, res, dy, ds, gamma, beta = data(N, D, dtype, D)
+    y, s, inv = A.fused_rms_norm_residual_op(x, res, gamma, epsilon=1e-5)
+    check_forward(x, res, gamma, 1e-5, y, s, inv)
+    dx, dg = A.fused_rms_norm_residual_grad_op(dy, ds, s, gamma, inv)
+    check_grad(dy, ds, s, gamma, inv, dx, dg)
+    _, s, mean, iv = A.fused_layer_norm_residual_op(x, res, gamma, beta, epsilon=1e-5)
+    dx, dg, db = A.fused_layer_norm_residual_grad_op(dy, ds, s, gamma, mean, iv)
+    check_grad(dy, ds, s, gamma, iv, dx, dg, mean, db)
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_another_device_than_the_current_one(lib):
+    x, res, dy, ds, gamma, _ = data(2000, 1024, "bf16", 4)
+    y, s, inv = A.fused_rms_norm_residual_op(x, res, gamma)
+    want = (y, s, inv, *A.fused_rms_norm_residual_grad_op(dy, ds, s, gamma, inv))
+    x, res, dy, ds, gamma = (t.to("cuda:1") for t in (x, res, dy, ds, gamma))
+    with torch.cuda.device(0):
+        y, s, inv = A.fused_rms_norm_residual_op(x, res, gamma)
+        got = (y, s, inv, *A.fused_rms_norm_residual_grad_op(dy, ds, s, gamma, inv))
+    assert all(b.device.index == 1 and torch.equal(a, b.to(DEV)) for a, b in zip(want, got))
+    with pytest.raises(ValueError, match="residual is on"):
+        A.fused_rms_norm_residual_op(x, res.to(DEV), gamma)

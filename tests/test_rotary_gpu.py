@@ -562,3 +562,15 @@ def test_a_block_forward_and_backward(lib):
         # a few hundred roundings of 2^-24 along the way, sums of at most 192 terms
         assert float((p.grad.double() - w.grad).abs().max()) <= 1e-4 * float(w.grad.abs().max())
     assert lib.nvn_device_status() == _lib.NVN_OK
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_another_device_than_the_current_one(lib):
+    c = case(2, 300, 8, 2, 128, 64, "layer", False, "bf16", 4)
+    want = (*forward(c), *backward(c))
+    other = {k: v.to("cuda:1") if isinstance(v, torch.Tensor) else v for k, v in c.items()}
+    with torch.cuda.device(0):
+        got = (*forward(other), *backward(other))
+    assert all(b.device.index == 1 and torch.equal(a, b.to(DEV)) for a, b in zip(want, got))
+    with pytest.raises(ValueError, match="positions is on"):
+        forward(dict(other, positions=c["positions"]))
