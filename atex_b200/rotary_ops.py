@@ -76,8 +76,13 @@ def _on_cuda(t, name, device):
         raise ValueError(f"{name} is on {t.device}, q on {device}")
 
 
+def _readable(t):
+    """Whether the elements of a head are contiguous, so that the kernels take the view as it is."""
+    return t.stride(-1) == 1 or t.shape[-1] == 1
+
+
 def _rows_contiguous(t):
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    return t if _readable(t) else t.contiguous()
 
 
 def _checked_out(t, like, name):
@@ -152,18 +157,20 @@ class _Form:
             _on_cuda(t, name, q.device)
         # views that the kernels cannot read are copied at every call
         self.copies = not all(t is None or t.is_contiguous() for t in (*scales, *offsets, inv_freq, pair_axis))
-        self.copies = self.copies or any(t is not None and _rows_contiguous(t) is not t for t in (q, k))
+        self.copies = self.copies or any(t is not None and not _readable(t) for t in (q, k))
         self.empty = B * T == 0
         position_bytes = 8 if positions is None or positions.dtype == torch.int64 else 4
         self.head = (code, norm_code, int(interleaved), epsilon, B, T, D, pairs, axes, position_bytes)
         self.pos = pos
-        self.q = _layout(q)
-        self.k = (0, 0, 0, 0) if k is None else _layout(k)
         self.device, self.index = q.device, q.get_device()
-        # contiguous tensors of q's and k's shape: fresh outputs, and most gradients
+        # contiguous tensors of q's and k's shape: fresh outputs, copies, and most gradients
         self.q_shape, self.k_shape = q.shape, None if k is None else k.shape
         self.q_packed = (H, T * H * D, H * D, D)
         self.k_packed = None if k is None else (kh, T * kh * D, kh * D, D)
+        # what the kernels read, the copy's layout where there is one: the gradient's workspace
+        # follows from it
+        self.q = _layout(q) if _readable(q) else self.q_packed
+        self.k = (0, 0, 0, 0) if k is None else _layout(k) if _readable(k) else self.k_packed
         self.workspace = None
 
     def workspace_bytes(self, index):
@@ -209,15 +216,13 @@ def _problem(q, k, positions, inv_freq, pair_axis, scales, offsets, norm, interl
         if key is not None:
             _remember(_forms, key, form)
     params = (scales[0], offsets[0], scales[1], offsets[1])
-    layouts = form.q, form.k
     if form.copies:
         params = [None if t is None else t.contiguous() for t in params]
         inv_freq = None if inv_freq is None else inv_freq.contiguous()
         pair_axis = None if pair_axis is None else pair_axis.contiguous()
         q, k = _rows_contiguous(q), None if k is None else _rows_contiguous(k)
-        layouts = _layout(q), form.k if k is None else _layout(k)
     packed = _PROBLEM.pack(*form.head, _ptr(positions), *form.pos, _ptr(inv_freq), _ptr(pair_axis), q.data_ptr(),
-                           *layouts[0], _ptr(k), *layouts[1], *[_ptr(t) for t in params])
+                           *form.q, _ptr(k), *form.k, *[_ptr(t) for t in params])
     # the copies must outlive the launch that reads them
     return form, packed, q, k, (params, inv_freq, pair_axis)
 

@@ -1,0 +1,48 @@
+"""The operators of a transformer block at the edges of what their documentation allows."""
+import pytest
+import torch
+
+import atex_b200 as A
+from atex_b200 import testing as T
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+U = 2.0 ** -24
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+# ---------------------------------------------------------------------------
+# gradients of views whose heads are not contiguous: the call copies them
+# ---------------------------------------------------------------------------
+def transposed(t):
+    """The same values with the heads, and not the elements of a head, contiguous."""
+    return t.transpose(-1, -2).contiguous().transpose(-1, -2)
+
+
+@pytest.mark.parametrize("norm", ["rms", "layer"])
+@pytest.mark.parametrize("B,T_,dtype", [(1, 300, "bf16"), (2, 2048, "f16"), (1, 2048, "f32")])
+def test_gradient_of_views_that_are_copied(lib, B, T_, dtype, norm):
+    hq, hk, hd = 32, 8, 128
+    g, dt = gen(B + T_), T.TORCH_DTYPE[dtype]
+
+    def r(*shape):
+        return torch.randn(*shape, generator=g, device=DEV).to(dt)
+    q, k, dq, dk = r(B, T_, hq, hd), r(B, T_, hk, hd), r(B, T_, hq, hd), r(B, T_, hk, hd)
+    sq, sk = (torch.rand(hd, generator=g, device=DEV) + 0.5 for _ in range(2))
+    off = (sq - 1, sk - 1) if norm == "layer" else (None, None)
+    f, ax = A.rotary_frequencies((16, 24, 24), device=DEV)
+    pos = torch.randint(0, 1000, (3, B, T_), generator=g, device=DEV)
+    want = A.fused_head_norm_rotary_grad_op(dq, dk, q, k, pos, f, ax, sq, sk, norm=norm)
+    qt, kt = transposed(q), transposed(k)
+    assert qt.stride(-1) == hq and kt.stride(-1) == hk
+    for a, b in ((qt, kt), (qt, k), (q, kt)):
+        got = A.fused_head_norm_rotary_grad_op(dq, dk, a, b, pos, f, ax, sq, sk, norm=norm)
+        assert all(y is None or torch.equal(x, y) for x, y in zip(got, want))
+    leaves = [t.detach().clone().requires_grad_() for t in (qt, kt)]
+    assert leaves[0].stride(-1) == hq
+    out = A.head_norm_rotary(*leaves, pos, f, ax, sq, sk, *off, norm=norm)
+    torch.autograd.backward(out, [dq, dk])
+    assert torch.equal(leaves[0].grad, want[0]) and torch.equal(leaves[1].grad, want[1])
