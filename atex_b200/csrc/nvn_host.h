@@ -132,6 +132,10 @@ inline cudaLaunchConfig_t dependent_launch_config(dim3 grid, dim3 block, size_t 
 // Remembers `e` for nvn_last_cuda_error() and clears it; returns NVN_ERR_CUDA.
 int fail_cuda(cudaError_t e);
 
+// The statistics of n rows without elements are not a number: a mean over nothing (all bits set
+// is a NaN).  `v` may be null.
+int empty_statistics(float* v, int64_t n, cudaStream_t s);
+
 inline bool aligned(const void* p, size_t a) {
   return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0;
 }

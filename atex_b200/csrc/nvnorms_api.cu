@@ -650,6 +650,12 @@ int fail_cuda(cudaError_t e) {
   return NVN_ERR_CUDA;
 }
 
+int empty_statistics(float* v, int64_t n, cudaStream_t s) {
+  if (v == nullptr || n == 0) return NVN_OK;
+  const cudaError_t e = cudaMemsetAsync(v, 0xff, static_cast<size_t>(n) * 4, s);
+  return e == cudaSuccess ? NVN_OK : fail_cuda(e);
+}
+
 int device_sm_count() {
   int v = g_sm_count.load(std::memory_order_relaxed);
   if (v > 0) return v;

@@ -168,7 +168,7 @@ extern "C" {
 int nvn_rms_fwd(int dtype, const void* x, const float* gamma, int64_t N, int64_t D, float epsilon,
                 void* y, float* inv_rms, void* stream) {
   if (!valid_dtype(dtype) || N < 0 || D < 0) return NVN_ERR_INVALID_ARGUMENT;
-  if (N == 0 || D == 0) return NVN_OK;
+  if (N == 0 || D == 0) return empty_statistics(inv_rms, N, static_cast<cudaStream_t>(stream));
   if (x == nullptr || gamma == nullptr || y == nullptr) return NVN_ERR_INVALID_ARGUMENT;
   return forward(dtype, x, nullptr, gamma, N, D, epsilon, nullptr, y, inv_rms,
                  static_cast<cudaStream_t>(stream));
@@ -178,7 +178,7 @@ int nvn_rms_fwd_residual(int dtype, const void* x, const void* residual, const f
                          int64_t N, int64_t D, float epsilon, void* sum_out, void* y,
                          float* inv_rms, void* stream) {
   if (!valid_dtype(dtype) || N < 0 || D < 0) return NVN_ERR_INVALID_ARGUMENT;
-  if (N == 0 || D == 0) return NVN_OK;
+  if (N == 0 || D == 0) return empty_statistics(inv_rms, N, static_cast<cudaStream_t>(stream));
   if (x == nullptr || residual == nullptr || gamma == nullptr || sum_out == nullptr || y == nullptr ||
       sum_out == y)
     return NVN_ERR_INVALID_ARGUMENT;

@@ -179,7 +179,8 @@ NVN_API int nvn_ln_bwd_residual(int dtype, const void* dy, const void* dsum, con
  *   y_ij      = x_ij inv_rms_i gamma_j
  * y may alias x.  No workspace.  The residual form normalises s_ij = T(x_ij + residual_ij),
  * which it also writes; sum_out may alias x or residual, y may alias x or residual, and
- * sum_out and y must not overlap.  Rows of any width.  No counterpart in the reference. */
+ * sum_out and y must not overlap.  Rows of any width; D = 0 leaves NaN in inv_rms, the mean of
+ * nothing.  No counterpart in the reference. */
 NVN_API int nvn_rms_fwd(int dtype, const void* x, const float* gamma, int64_t N, int64_t D,
                         float epsilon, void* y, float* inv_rms, void* stream);
 NVN_API int nvn_rms_fwd_residual(int dtype, const void* x, const void* residual,

@@ -46,3 +46,16 @@ def test_gradient_of_views_that_are_copied(lib, B, T_, dtype, norm):
     out = A.head_norm_rotary(*leaves, pos, f, ax, sq, sk, *off, norm=norm)
     torch.autograd.backward(out, [dq, dk])
     assert torch.equal(leaves[0].grad, want[0]) and torch.equal(leaves[1].grad, want[1])
+
+
+# ---------------------------------------------------------------------------
+# RMS rows of no elements
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_statistics_of_rows_without_elements(lib, dtype):
+    """The mean of nothing is not a number; the buffer's former content is not an answer."""
+    x, g = torch.empty(5, 0, dtype=T.TORCH_DTYPE[dtype], device=DEV), torch.ones(0, device=DEV)
+    stats = torch.full((5,), 7.0, device=DEV)
+    assert torch.isnan(A.fused_rms_norm_op(x, g, out_stats=stats)[1]).all() and torch.isnan(stats).all()
+    stats.fill_(7.0)
+    assert torch.isnan(A.fused_rms_norm_residual_op(x, x, g, out_stats=stats)[2]).all()
