@@ -635,6 +635,12 @@ int run_nlc(int dtype, bool bwd, const void* dy, const void* x, const float* gam
   return NVN_OK;
 }
 
+// Both statistics of n rows without elements.
+int empty_statistics(float* mean, float* inv_std, int64_t n, cudaStream_t stream) {
+  const int st = nvn::empty_statistics(mean, n, stream);
+  return st != NVN_OK ? st : nvn::empty_statistics(inv_std, n, stream);
+}
+
 int zero_grads(float* dgamma, float* dbeta, int64_t F, cudaStream_t stream) {
   if (F <= 0) return NVN_OK;
   cudaError_t e = cudaMemsetAsync(dgamma, 0, static_cast<size_t>(F) * 4, stream);
@@ -857,7 +863,7 @@ int nvn_ln_fwd(int dtype, const void* x, const float* gamma, const float* beta, 
                int64_t D, float epsilon, void* y, float* mean, float* inv_std, void* workspace,
                size_t workspace_bytes, void* stream) {
   if (!valid_dtype(dtype) || N < 0 || D < 0) return NVN_ERR_INVALID_ARGUMENT;
-  if (N == 0 || D == 0) return NVN_OK;
+  if (N == 0 || D == 0) return empty_statistics(mean, inv_std, N, static_cast<cudaStream_t>(stream));
   if (x == nullptr || gamma == nullptr || beta == nullptr || y == nullptr || mean == nullptr ||
       inv_std == nullptr)
     return NVN_ERR_INVALID_ARGUMENT;
@@ -871,7 +877,7 @@ int nvn_ln_fwd_residual(int dtype, const void* x, const void* residual, const fl
                         void* y, float* mean, float* inv_std, void* workspace,
                         size_t workspace_bytes, void* stream) {
   if (!valid_dtype(dtype) || N < 0 || D < 0) return NVN_ERR_INVALID_ARGUMENT;
-  if (N == 0 || D == 0) return NVN_OK;
+  if (N == 0 || D == 0) return empty_statistics(mean, inv_std, N, static_cast<cudaStream_t>(stream));
   if (x == nullptr || residual == nullptr || gamma == nullptr || beta == nullptr ||
       sum_out == nullptr || y == nullptr || mean == nullptr || inv_std == nullptr)
     return NVN_ERR_INVALID_ARGUMENT;
@@ -967,7 +973,8 @@ int nvn_in_fwd(int dtype, const void* x, const float* gamma, const float* beta, 
                int64_t C, int64_t D, int channel_first, float epsilon, void* y, float* mean,
                float* inv_std, void* workspace, size_t workspace_bytes, void* stream) {
   if (!valid_dtype(dtype) || N < 0 || C < 0 || D < 0) return NVN_ERR_INVALID_ARGUMENT;
-  if (N == 0 || C == 0 || D == 0) return NVN_OK;
+  if (N == 0 || C == 0 || D == 0)
+    return empty_statistics(mean, inv_std, N * C, static_cast<cudaStream_t>(stream));
   if (x == nullptr || gamma == nullptr || beta == nullptr || y == nullptr || mean == nullptr ||
       inv_std == nullptr)
     return NVN_ERR_INVALID_ARGUMENT;

@@ -29,9 +29,10 @@
  *   - The second saved statistic is 1/sqrt(var + epsilon) (the reference calls it
  *     "inv_var", norm_util.h:255-258).
  *   - Backward uses the mean / inverse-std passed in; it never recomputes them.
- *   - Empty inputs (N*D == 0 or N*C*D == 0) launch nothing, except that backward
- *     zero-fills dgamma / dbeta (the reference's CPU kernels do,
- *     fused_layer_norm_op.cc:96-103; its GPU kernels leave them unwritten).
+ *   - Empty inputs (N*D == 0 or N*C*D == 0) launch no kernel.  Backward zero-fills dgamma /
+ *     dbeta (the reference's CPU kernels do, fused_layer_norm_op.cc:96-103; its GPU kernels
+ *     leave them unwritten); forward fills the statistics of rows that have no elements with
+ *     NaN, the mean of nothing.
  *   - Calls are re-entrant and thread-safe.
  */
 #ifndef NVNORMS_H_

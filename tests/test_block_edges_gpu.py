@@ -59,3 +59,25 @@ def test_statistics_of_rows_without_elements(lib, dtype):
     assert torch.isnan(A.fused_rms_norm_op(x, g, out_stats=stats)[1]).all() and torch.isnan(stats).all()
     stats.fill_(7.0)
     assert torch.isnan(A.fused_rms_norm_residual_op(x, x, g, out_stats=stats)[2]).all()
+
+
+# ---------------------------------------------------------------------------
+# LayerNorm and InstanceNorm of no elements
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_layer_norm_statistics_of_rows_without_elements(lib, dtype):
+    x, g = torch.empty(5, 0, dtype=T.TORCH_DTYPE[dtype], device=DEV), torch.ones(0, device=DEV)
+    stats = torch.full((2, 5), 7.0, device=DEV)
+    A.fused_layer_norm_op(x, g, g, out_stats=(stats[0], stats[1]))
+    assert torch.isnan(stats).all()
+    stats.fill_(7.0)
+    A.fused_layer_norm_residual_op(x, x, g, g, out_stats=(stats[0], stats[1]))
+    assert torch.isnan(stats).all()
+
+
+@pytest.mark.parametrize("shape,fmt", [((3, 2, 0, 4), "NC..."), ((3, 0, 4, 2), "N...C")])
+def test_instance_norm_statistics_of_items_without_elements(lib, shape, fmt):
+    x, g = torch.empty(shape, device=DEV), torch.ones(2, device=DEV)
+    stats = torch.full((2, 3, 2), 7.0, device=DEV)
+    A.fused_instance_norm_op(x, g, g, data_format=fmt, out_stats=(stats[0], stats[1]))
+    assert torch.isnan(stats).all()
