@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 from typing import Iterable, List, Sequence, Tuple
 
 import torch
@@ -432,6 +433,22 @@ def fused_instance_norm_grad_op(y_backprop, x, scale, reserve_space_1, reserve_s
                                    ws_bytes, grad_exchange.next_comm(C), stream)
     _check(st, "nvn_in_bwd")
     return dx, dgamma, dbeta
+
+
+def _first_derivatives_only(backward):
+    """For the backward of an autograd function whose gradient op has no gradient of its own: under
+    create_graph its results raise when they are differentiated again.  (torch's
+    once_differentiable leaves them constant when the incoming gradients do not require one, although
+    they depend on the saved inputs as well.)"""
+    @functools.wraps(backward)
+    def wrapped(ctx, *grads):
+        if not torch.is_grad_enabled():
+            return backward(ctx, *grads)
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        refuse = torch._C._functions.DelayedError(b"the fused norm ops have first derivatives only", len(out))
+        return refuse(*[None if t is None else t.detach().requires_grad_() for t in out])
+    return wrapped
 
 
 # ---------------------------------------------------------------------------

@@ -24,8 +24,8 @@ import torch
 
 from . import _lib
 from .nv_norm_ops import (InvalidArgumentError, LayerNormalization, _axis_list, _check, _dtype_code,
-                          _grad_outputs, _like_output, _ln_dims, _on_device, _param, _remember,
-                          _require, fused_layer_norm_grad_op,
+                          _first_derivatives_only, _grad_outputs, _like_output, _ln_dims, _on_device,
+                          _param, _remember, _require, fused_layer_norm_grad_op,
                           fused_layer_norm_residual_op)
 
 __all__ = [
@@ -254,6 +254,7 @@ class _rms_norm_grad(torch.autograd.Function):
         return y
 
     @staticmethod
+    @_first_derivatives_only
     def backward(ctx, grad_y):
         x, gamma, inv = ctx.saved_tensors
         dx, dgamma = fused_rms_norm_grad_op(grad_y, x, gamma, inv, axis=ctx.axis)
@@ -271,9 +272,14 @@ class _rms_norm_residual_grad(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_y, grad_s):
-        s, gamma, inv = ctx.saved_tensors
-        if grad_y is None:   # only the sum was used
+        if grad_y is None:   # only the sum was used: its gradient passes, with whatever graph it has
             return grad_s, grad_s, None, None, None
+        return _rms_norm_residual_grad.through_norm(ctx, grad_y, grad_s)
+
+    @staticmethod
+    @_first_derivatives_only
+    def through_norm(ctx, grad_y, grad_s):
+        s, gamma, inv = ctx.saved_tensors
         dx, dgamma = _rms_grad(grad_y, grad_s, s, gamma, inv, ctx.axis, None, None)
         return dx, dx, dgamma, None, None
 
@@ -289,9 +295,14 @@ class _layer_norm_residual_grad(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_y, grad_s):
-        s, gamma, mean, inv = ctx.saved_tensors
         if grad_y is None:
             return grad_s, grad_s, None, None, None, None
+        return _layer_norm_residual_grad.through_norm(ctx, grad_y, grad_s)
+
+    @staticmethod
+    @_first_derivatives_only
+    def through_norm(ctx, grad_y, grad_s):
+        s, gamma, mean, inv = ctx.saved_tensors
         if grad_s is None:
             dx, dgamma, dbeta = fused_layer_norm_grad_op(grad_y, s, gamma, mean, inv, axis=ctx.axis)
         else:

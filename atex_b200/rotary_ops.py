@@ -26,7 +26,8 @@ from typing import Sequence, Tuple
 import torch
 
 from . import _lib
-from .nv_norm_ops import InvalidArgumentError, _check, _dtype_code, _param, _remember, _require
+from .nv_norm_ops import (InvalidArgumentError, _check, _dtype_code, _first_derivatives_only, _param, _remember,
+                          _require)
 from .rms_norm_ops import _on_stream, _scratch
 
 __all__ = ["fused_head_norm_rotary_op", "fused_head_norm_rotary_grad_op", "head_norm_rotary",
@@ -334,6 +335,7 @@ class _head_norm_rotary_grad(torch.autograd.Function):
         return out
 
     @staticmethod
+    @_first_derivatives_only
     def backward(ctx, grad_q, grad_k):
         q, k, scale_q, scale_k, positions, inv_freq, pair_axis = ctx.saved_tensors
         if grad_q is None:

@@ -81,3 +81,55 @@ def test_instance_norm_statistics_of_items_without_elements(lib, shape, fmt):
     stats = torch.full((2, 3, 2), 7.0, device=DEV)
     A.fused_instance_norm_op(x, g, g, data_format=fmt, out_stats=(stats[0], stats[1]))
     assert torch.isnan(stats).all()
+
+
+# ---------------------------------------------------------------------------
+# second derivatives: refused, not silently left out
+# ---------------------------------------------------------------------------
+def differentiable_calls():
+    g = gen(3)
+    x, r = torch.randn(6, 64, generator=g, device=DEV), torch.randn(6, 64, generator=g, device=DEV)
+    w, b = torch.rand(64, generator=g, device=DEV) + 0.5, torch.randn(64, generator=g, device=DEV)
+    q, k = torch.randn(1, 3, 2, 64, generator=g, device=DEV), torch.randn(1, 3, 1, 64, generator=g, device=DEV)
+    f, ax = A.rotary_frequencies((32,), device=DEV)
+    pos = torch.arange(3, device=DEV)[None]
+    return {
+        "rms": (x, lambda t: A.rms_norm(t, w)),
+        "rms_residual": (x, lambda t: A.rms_norm_residual(t, r, w)[0]),
+        "rms_residual_both": (x, lambda t: sum(A.rms_norm_residual(t, r, w))),
+        "layer_residual": (x, lambda t: A.layer_norm_residual(t, r, w, b)[0]),
+        "layer_residual_both": (x, lambda t: sum(A.layer_norm_residual(t, r, w, b))),
+        "rotary": (q, lambda t: A.head_norm_rotary(t, k, pos, f, ax, w, w)[0]),
+        "rotary_none": (q, lambda t: A.head_norm_rotary(t, None, pos, f, ax, norm="none")[0]),
+    }
+
+
+@pytest.mark.parametrize("name", ["rms", "rms_residual", "rms_residual_both", "layer_residual", "layer_residual_both",
+                                  "rotary", "rotary_none"])
+def test_second_derivatives_are_refused(lib, name):
+    x, call = differentiable_calls()[name]
+    up = torch.randn(x.shape, generator=gen(4), device=DEV)
+    a = x.clone().requires_grad_()
+    want, = torch.autograd.grad(call(a), a, up)
+    for grads_too in (False, True):
+        a, u = x.clone().requires_grad_(), up.clone().requires_grad_(grads_too)
+        got, = torch.autograd.grad(call(a), a, u, create_graph=True)
+        assert torch.equal(got, want)     # the first derivative is there
+        with pytest.raises(RuntimeError, match="first derivatives only"):
+            (got * up).sum().backward()   # of the gradient itself
+        a = x.clone().requires_grad_()
+        got, = torch.autograd.grad(call(a) * a.detach() + a * a, a, up, create_graph=True)
+        with pytest.raises(RuntimeError, match="first derivatives only"):
+            got.square().sum().backward()   # beside a part that has one
+
+
+def test_second_derivatives_of_the_sum_alone(lib):
+    """The sum passes its gradient on unchanged, so what is built on that gradient has a derivative."""
+    g = gen(5)
+    x, r = (torch.randn(6, 64, generator=g, device=DEV) for _ in range(2))
+    w = torch.ones(64, device=DEV)
+    for call in (lambda a: A.rms_norm_residual(a, r, w)[1], lambda a: A.layer_norm_residual(a, r, w, w)[1]):
+        a = x.clone().requires_grad_()
+        first, = torch.autograd.grad((call(a) ** 3).sum(), a, create_graph=True)
+        second, = torch.autograd.grad(first.sum(), a)
+        assert torch.allclose(second, 6 * (x + r), rtol=1e-6)
