@@ -467,6 +467,7 @@ class _layer_norm_grad(torch.autograd.Function):
         return y, mean, inv_std
 
     @staticmethod
+    @_first_derivatives_only
     def backward(ctx, grad_y, _gm, _gi):
         x, gamma, mean, inv_std = ctx.saved_tensors
         dx, dgamma, dbeta = fused_layer_norm_grad_op(grad_y, x, gamma, mean, inv_std, axis=ctx.axis)
@@ -486,6 +487,7 @@ class _instance_norm_grad(torch.autograd.Function):
         return y, mean, inv_std
 
     @staticmethod
+    @_first_derivatives_only
     def backward(ctx, grad_y, _gm, _gi):
         x, gamma, mean, inv_std = ctx.saved_tensors
         dx, dgamma, dbeta = fused_instance_norm_grad_op(grad_y, x, gamma, mean, inv_std,

@@ -133,3 +133,25 @@ def test_second_derivatives_of_the_sum_alone(lib):
         first, = torch.autograd.grad((call(a) ** 3).sum(), a, create_graph=True)
         second, = torch.autograd.grad(first.sum(), a)
         assert torch.allclose(second, 6 * (x + r), rtol=1e-6)
+
+
+# ---------------------------------------------------------------------------
+# the older functions' derivatives
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("name", ["layer", "instance"])
+def test_second_derivatives_of_layer_and_instance_norm_are_refused(lib, name):
+    """As in the reference, whose gradient ops have no gradient registered (nv_norm_ops.py:27-67)."""
+    g = gen(6)
+    x = torch.randn(3, 5, 4, 8, generator=g, device=DEV)
+    w = torch.rand(8, generator=g, device=DEV) + 0.5
+    up = torch.randn(x.shape, generator=g, device=DEV)
+
+    def call(t):
+        return A.layer_norm(t, w, w) if name == "layer" else A.instance_norm(t, w, w)
+    a = x.clone().requires_grad_()
+    want, = torch.autograd.grad(call(a), a, up)
+    a = x.clone().requires_grad_()
+    got, = torch.autograd.grad(call(a), a, up, create_graph=True)
+    assert torch.equal(got, want)
+    with pytest.raises(RuntimeError, match="first derivatives only"):
+        (got * got + a).sum().backward()
