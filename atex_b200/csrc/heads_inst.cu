@@ -98,16 +98,16 @@ cudaError_t launch_kernel(HeadArgs a, cudaStream_t s, bool dry_run, HeadPlan* pl
   });
   if (e != cudaSuccess) return e;
   // persistent: tables and (backward) the parameter sums of a CTA serve all its tiles
-  static std::atomic<int64_t> cached{0};  // (shared bytes << 20) | CTAs per SM
-  const int64_t c = cached.load(std::memory_order_relaxed);
-  int per_sm = 0;
-  if (c != 0 && static_cast<size_t>(c >> 20) == smem) {
-    per_sm = static_cast<int>(c & 0xfffff);
-  } else {
+  static ResidencyCache resident_per_sm;   // CTAs per SM, by shared bytes
+  int dev = 0;
+  e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  int per_sm = resident_per_sm.get(dev, smem);
+  if (per_sm == 0) {
     e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, BLOCK, smem);
     if (e != cudaSuccess) return e;
     if (per_sm < 1) per_sm = 1;
-    cached.store((static_cast<int64_t>(smem) << 20) | per_sm, std::memory_order_relaxed);
+    resident_per_sm.put(dev, smem, per_sm);
   }
   const int64_t resident = static_cast<int64_t>(per_sm) * device_sm_count();
   const int64_t grid = a.tiles < resident ? a.tiles : resident;

@@ -191,6 +191,21 @@ inline cudaError_t once_per_device(std::atomic<uint64_t>& mask, F&& set) {
   if (bit != 0) mask.fetch_or(bit, std::memory_order_release);
   return cudaSuccess;
 }
+// What a launcher remembers of its kernel's residency: a count below 2^20 for one key (bytes of
+// dynamic shared memory) per device, because SM counts may differ.  A key that changes from call
+// to call is asked for again; ordinals beyond 63 always are.
+struct ResidencyCache {
+  std::atomic<int64_t> slot[64] = {};   // (key << 20) | count
+  int get(int dev, size_t key) const {  // 0: not known
+    const int64_t c = dev >= 0 && dev < 64 ? slot[dev].load(std::memory_order_relaxed) : 0;
+    return c != 0 && static_cast<size_t>(c >> 20) == key ? static_cast<int>(c & 0xfffff) : 0;
+  }
+  void put(int dev, size_t key, int count) {
+    if (dev >= 0 && dev < 64)
+      slot[dev].store((static_cast<int64_t>(key) << 20) | count, std::memory_order_relaxed);
+  }
+};
+
 // Device address of the library's status word on the current device (nullptr on failure).
 int* device_status_word();
 

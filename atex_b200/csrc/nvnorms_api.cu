@@ -28,7 +28,7 @@ namespace nvn {
 namespace {
 std::atomic<uint64_t> g_launches{0};
 thread_local int t_last_cuda_error = 0;
-std::atomic<int> g_sm_count{0};
+std::atomic<int> g_sm_count[64] = {};   // per device ordinal
 
 struct Shape {
   int tpr, vpt, cs, pf;
@@ -663,15 +663,17 @@ int empty_statistics(float* v, int64_t n, cudaStream_t s) {
 }
 
 int device_sm_count() {
-  int v = g_sm_count.load(std::memory_order_relaxed);
+  int dev = 0, v = 0;
+  const bool known = cudaGetDevice(&dev) == cudaSuccess;
+  const bool kept = known && dev >= 0 && dev < 64;
+  if (kept) v = g_sm_count[dev].load(std::memory_order_relaxed);
   if (v > 0) return v;
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
+  if (!known ||
       cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v <= 0) {
     (void)cudaGetLastError();
     return 148;  // B200; only reached when no device is usable
   }
-  g_sm_count.store(v, std::memory_order_relaxed);
+  if (kept) g_sm_count[dev].store(v, std::memory_order_relaxed);
   return v;
 }
 

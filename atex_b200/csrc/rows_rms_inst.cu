@@ -60,7 +60,7 @@ cudaError_t launch_exact(const RowsResArgs& a, cudaStream_t stream, bool dry_run
   } else {
     kernel = rows_fwd_kernel<T, EPV, TPR, VPT, 1, RB, PR, MINB, PF, EXACT, false, THIRD, true>;
   }
-  static std::atomic<int64_t> cached{0};  // (ring bytes << 20) | resident CTAs
+  static ResidencyCache resident;   // CTAs on the device, by ring bytes
   static std::atomic<uint64_t> prepared{0};
   if constexpr (TMA) {
     const cudaError_t e = once_per_device(prepared, [&]() -> cudaError_t {
@@ -74,13 +74,12 @@ cudaError_t launch_exact(const RowsResArgs& a, cudaStream_t stream, bool dry_run
     });
     if (e != cudaSuccess) return e;
   }
-  int units = 0;
-  const int64_t c = cached.load(std::memory_order_relaxed);
-  if (c != 0 && static_cast<size_t>(c >> 20) == ring) {
-    units = static_cast<int>(c & 0xfffff);
-  } else {
+  int dev = -1;   // a size may be asked for without a device
+  if (cudaGetDevice(&dev) != cudaSuccess) (void)cudaGetLastError();
+  int units = resident.get(dev, ring);
+  if (units == 0) {
     units = resident_units(kernel, BLOCK, 1, ring);
-    cached.store((static_cast<int64_t>(ring) << 20) | units, std::memory_order_relaxed);
+    resident.put(dev, ring, units);
   }
   const int64_t need = (a.N + RPC * RB - 1) / (RPC * RB);
   const int64_t use = need < units ? need : units;

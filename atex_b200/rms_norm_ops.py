@@ -58,11 +58,12 @@ class _Rows:
         self.code, self.N, self.D, self.bytes = code, N, D, {}
 
     def workspace_bytes(self, fn_name: str, index: int) -> int:
-        """A size, asked for once with device `index` current."""
-        n = self.bytes.get(fn_name)
+        """A size, asked for once with device `index` current (it follows from the device's SMs)."""
+        n = self.bytes.get((fn_name, index))
         if n is None:
             with torch.cuda.device(index):
-                n = self.bytes[fn_name] = int(getattr(_lib.load(), fn_name)(self.code, self.N, self.D))
+                n = int(getattr(_lib.load(), fn_name)(self.code, self.N, self.D))
+            self.bytes[fn_name, index] = n
         return n
 
 

@@ -1,0 +1,67 @@
+"""The operators of a transformer block: host-side behaviour at the edges.  No GPU."""
+import contextlib
+import os
+import subprocess
+
+import pytest
+import torch
+
+from atex_b200 import _lib as L
+from atex_b200 import rms_norm_ops as M
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+# ---------------------------------------------------------------------------
+# sizes that follow from a device
+# ---------------------------------------------------------------------------
+def test_workspace_sizes_are_remembered_per_device(monkeypatch):
+    """A device with more SMs needs more partial rows."""
+    current, asked = [None], []
+
+    @contextlib.contextmanager
+    def device(index):
+        current[0] = index
+        yield
+
+    class Library:
+        @staticmethod
+        def nvn_rms_bwd_workspace_bytes(code, n, d):
+            asked.append(current[0])
+            return 256 * (1 + current[0])
+
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(L, "load", lambda: Library)
+    rows = M._Rows(0, 64, 128)
+    for _ in range(2):
+        assert rows.workspace_bytes("nvn_rms_bwd_workspace_bytes", 0) == 256
+        assert rows.workspace_bytes("nvn_rms_bwd_workspace_bytes", 3) == 1024
+    assert asked == [0, 3]
+
+
+def test_residency_is_remembered_per_device(tmp_path):
+    """The launchers' cache, compiled for the host."""
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    if not os.path.exists(os.path.join(cuda, "include", "cuda_runtime.h")):
+        pytest.skip("needs the CUDA headers")
+    src = tmp_path / "cache.cc"
+    src.write_text("""
+#include "nvn_host.h"
+static nvn::ResidencyCache c;
+int main() {
+  if (c.get(0, 0) != 0 || c.get(1, 4096) != 0) return 1;
+  c.put(0, 4096, 296);
+  if (c.get(0, 4096) != 296 || c.get(1, 4096) != 0 || c.get(0, 0) != 0) return 2;
+  c.put(1, 4096, 264);
+  if (c.get(0, 4096) != 296 || c.get(1, 4096) != 264) return 3;
+  c.put(0, 0, 148);
+  if (c.get(0, 0) != 148 || c.get(0, 4096) != 0 || c.get(1, 4096) != 264) return 4;
+  c.put(64, 4096, 7);
+  c.put(-1, 4096, 7);
+  return c.get(64, 4096) != 0 || c.get(-1, 4096) != 0 ? 5 : 0;
+}
+""")
+    exe = str(tmp_path / "cache")
+    subprocess.run(["g++", "-std=c++17", "-I", os.path.join(ROOT, "atex_b200", "csrc"), "-I", os.path.join(cuda, "include"),
+                    str(src), "-o", exe], check=True, capture_output=True, text=True)
+    assert subprocess.run([exe]).returncode == 0
