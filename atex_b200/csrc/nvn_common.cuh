@@ -42,6 +42,14 @@ struct Cvt<__nv_bfloat16> {
   }
 };
 
+__host__ __device__ constexpr int pow2_at_least(int n) { return n <= 1 ? 1 : 2 * pow2_at_least((n + 1) / 2); }
+
+constexpr float kMaxFloat = 3.402823466e38f;
+
+// Whether sums of squares of T can pass fp32's end (an fp16 value squares to 4.3e9 at most).
+template <typename T>
+constexpr bool kSquaresOverflow = !std::is_same<T, __half>::value;
+
 // Elements of T in one 128-bit access.
 template <typename T>
 struct VecTraits {

@@ -32,6 +32,12 @@ __global__ void __launch_bounds__(kRowBlock) rms_generic_fwd_kernel(const RowsRe
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t rowvecs = a.D / EPV;
   const float inv_D = 1.0f / static_cast<float>(a.D);
+  // squares are scaled down by a power of two, at least as many as a thread adds: see rows_fwd_kernel
+  float squares = 1.f;
+  if constexpr (kSquaresOverflow<T>) {
+    for (int64_t n = (rowvecs + kRowBlock - 1) / kRowBlock * EPV; n > 1; n = (n + 1) / 2) squares *= 2.f;
+  }
+  const E down = M::bcast(1.f / squares);
   for (int64_t row = blockIdx.x; row < a.N; row += gridDim.x) {
     const P* xp = reinterpret_cast<const P*>(a.x) + row * rowvecs;
     const P* rp = reinterpret_cast<const P*>(a.res) + (RES ? row * rowvecs : 0);
@@ -51,14 +57,14 @@ __global__ void __launch_bounds__(kRowBlock) rms_generic_fwd_kernel(const RowsRe
         unpack<T, EPV>(s, v);
       }
 #pragma unroll
-      for (int e = 0; e < NE; ++e) acc = M::fma(v[e], v[e], acc);
+      for (int e = 0; e < NE; ++e) acc = M::fma(kSquaresOverflow<T> ? M::mul(v[e], down) : v[e], v[e], acc);
     }
-    float q[1] = {M::hsum(acc) * inv_D};  // the thread's share of the mean: see rows_fwd_kernel
+    float q[1] = {M::hsum(acc) * (inv_D * squares)};  // the thread's share of the mean: see rows_fwd_kernel
+    // the thread reads back only what it wrote itself (s), or what nobody has written (x)
+    const P* back = RES ? sp : xp;
     group_allreduce<1, kRowBlock, kRowBlock, 1>(q, sm, phase, warp, lane);
     const float inv = rsqrtf(q[0] + a.eps);
     const E iv2 = M::bcast(inv);
-    // the thread reads back only what it wrote itself (s), or what nobody has written (x)
-    const P* back = RES ? sp : xp;
     for (int64_t i = tid; i < rowvecs; i += kRowBlock) {
       E v[NE], g[NE];
       unpack<T, EPV>(load_keep<T, EPV>(reinterpret_cast<const T*>(back + i)), v);

@@ -155,3 +155,37 @@ def test_second_derivatives_of_layer_and_instance_norm_are_refused(lib, name):
     assert torch.equal(got, want)
     with pytest.raises(RuntimeError, match="first derivatives only"):
         (got * got + a).sum().backward()
+
+
+# ---------------------------------------------------------------------------
+# wide rows whose mean square is near fp32's end
+# ---------------------------------------------------------------------------
+def huge(shape, dtype, seed, top):
+    """Magnitudes top to top / 16 with both signs, the root mean square at most top."""
+    g = gen(seed)
+    m = torch.exp2(-4 * torch.rand(shape, generator=g, device=DEV))
+    m[..., ::3] = 1.0
+    sign = torch.randint(0, 2, shape, generator=g, device=DEV) * 2 - 1
+    return (m * sign * top).to(T.TORCH_DTYPE[dtype])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("D", [1, 5, 64, 100, 512, 1001, 1024, 2044, 4096, 8192, 16384, 20001, 40000])
+def test_rms_of_rows_whose_mean_square_just_fits(lib, dtype, D):
+    """1.8e19 squared is 3.24e38, of 3.40e38 that fp32 holds: mean squares fit, sums of two do not.
+    The bounds are those of every row, with two roundings more for the scaled squares and their
+    scale, (64 + D / 512) / 2 + 12 units of 2^-24; the squares of the small values, scaled down by a
+    power of two, are far from fp32's lower end."""
+    for N in (1, 40):
+        x = huge((N, D), dtype, D + N, 1.8e19)
+        gamma = torch.rand(D, generator=gen(D), device=DEV) + 0.5
+        x64 = x.double()
+        inv64 = 1 / torch.sqrt((x64 * x64).mean(1) + 1e-5)
+        want = x64 * inv64[:, None] * gamma.double()
+        allow = U * ((64 + D / 512) / 2 + 12)
+        half = torch.finfo(x.dtype).eps / 2 if dtype != "f32" else 0.0
+        zero = torch.zeros_like(x)
+        for y, inv in (A.fused_rms_norm_op(x, gamma, epsilon=1e-5),
+                       A.fused_rms_norm_residual_op(x, zero, gamma, epsilon=1e-5)[::2]):
+            assert ((inv.double() - inv64).abs() <= allow * inv64).all()
+            assert ((y.double() - want).abs() <= (allow + half * 1.001) * want.abs()).all()
