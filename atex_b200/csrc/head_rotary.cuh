@@ -587,6 +587,9 @@ __global__ void __launch_bounds__(head_block(R), head_ctas(BWD, R, NORM, PAD)) h
         if constexpr (NORM != 0) {
           // sum of squares; backward: sum gy c and, for mean and variance, sum gy beside it
           constexpr int NR = BWD ? NORM + 1 : 1;
+          // squares scaled down by a power of two, as many as a lane adds at once: see rows_fwd_kernel
+          constexpr float kSquares = kSquaresOverflow<T> ? 2 * V : 1;
+          const E down = M::bcast(1.f / kSquares);
           float red[NR * R];
 #pragma unroll
           for (int r = 0; r < R; ++r) {
@@ -601,7 +604,7 @@ __global__ void __launch_bounds__(head_block(R), head_ctas(BWD, R, NORM, PAD)) h
               for (int k = 0; k < 2; ++k)
 #pragma unroll
                 for (int e = 0; e < NE; ++e) {
-                  acc[0] = M::fma(x[r][i][k][e], x[r][i][k][e], acc[0]);
+                  acc[0] = M::fma(kSquares > 1.f ? M::mul(x[r][i][k][e], down) : x[r][i][k][e], x[r][i][k][e], acc[0]);
                   if constexpr (BWD) {
                     const E gy = M::mul(d[r][i][k][e], g[i][k][e]);
                     acc[1] = M::fma(gy, x[r][i][k][e], acc[1]);
@@ -610,7 +613,7 @@ __global__ void __launch_bounds__(head_block(R), head_ctas(BWD, R, NORM, PAD)) h
                 }
 #pragma unroll
               for (int k = 0; k < NR; ++k)   // shares of means: no overflow in the sum
-                if (ok[i]) red[r * NR + k] += M::hsum(acc[k]) * a.inv_hd;
+                if (ok[i]) red[r * NR + k] += M::hsum(acc[k]) * (k == 0 ? a.inv_hd * kSquares : a.inv_hd);
             }
           }
           head_reduce<FULL>(red, tph);

@@ -189,3 +189,41 @@ def test_rms_of_rows_whose_mean_square_just_fits(lib, dtype, D):
                        A.fused_rms_norm_residual_op(x, zero, gamma, epsilon=1e-5)[::2]):
             assert ((inv.double() - inv64).abs() <= allow * inv64).all()
             assert ((y.double() - want).abs() <= (allow + half * 1.001) * want.abs()).all()
+
+
+# ---------------------------------------------------------------------------
+# narrow heads whose mean square is near fp32's end
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("hd,rows", [(1, 5), (7, 50), (33, 50), (64, 5), (64, 4000), (80, 3000), (128, 7), (128, 3000),
+                                     (256, 1500), (320, 40), (511, 40)])
+@pytest.mark.parametrize("norm", ["rms", "layer"])
+def test_heads_whose_mean_square_just_fits(lib, dtype, hd, rows, norm):
+    """Forward: 40 units of 2^-24 of the magnitudes, as for every head, and two more for the scaled
+    squares.  For a norm with mean the values are 0.9e19, so that a value less the mean, at most 1.8e19,
+    squares to no more than fits, and a sum of 16 of them is far below fp32's end."""
+    top = 1.8e19 if norm == "rms" else 0.9e19
+    q = huge((1, rows, 2, hd), dtype, hd + rows, top)
+    scale = torch.rand(hd, generator=gen(hd), device=DEV) + 0.5
+    off = torch.zeros(hd, device=DEV) if norm == "layer" else None
+    x = q.double()
+    c = x - x.mean(-1, keepdim=True) if norm == "layer" else x
+    mag = x.abs() + x.abs().mean(-1, keepdim=True) if norm == "layer" else x.abs()
+    inv = 1 / torch.sqrt((c * c).mean(-1, keepdim=True) + 1e-6)
+    half = torch.finfo(q.dtype).eps / 2 if dtype != "f32" else 0.0
+    y, _ = A.fused_head_norm_rotary_op(q, None, None, scale_q=scale, offset_q=off, norm=norm, epsilon=1e-6)
+    want = c * inv * scale.double()
+    assert ((y.double() - want).abs() <= 42 * U * mag * inv * scale.double() + half * 1.001 * want.abs()).all()
+    # the gradient forms the statistics again; its terms are 1 / 1e19 and their products with c of order one
+    dy = torch.randn(q.shape, generator=gen(9), device=DEV).to(q.dtype)
+    dx, _, dscale, _, _, _ = A.fused_head_norm_rotary_grad_op(dy, None, q, None, None, scale_q=scale, norm=norm,
+                                                              epsilon=1e-6)
+    xh, xm = c * inv, mag * inv
+    gy = dy.double() * scale.double()
+    lift = gy.mean(-1, keepdim=True) if norm == "layer" else 0.0
+    want = inv * (gy - lift - xh * (gy * xh).mean(-1, keepdim=True))
+    big = inv * (gy.abs() + gy.abs().mean(-1, keepdim=True) + xm * (gy.abs() * xm).mean(-1, keepdim=True))
+    assert ((dx.double() - want).abs() <= 98 * U * big + half * 1.001 * want.abs()).all()
+    terms = dy.double() * xh
+    allow = U * (34 + 64 + 2 * rows / 16) * (dy.double().abs() * xm).sum((0, 1, 2))
+    assert ((dscale.double() - terms.sum((0, 1, 2))).abs() <= allow).all()
