@@ -142,8 +142,29 @@ __global__ void __launch_bounds__(kColBlock)
   load_param_lanes<EPV>(a.gamma, vec * EPV, g);
 #pragma unroll
   for (int e = 0; e < NE; ++e) dg[e] = db[e] = M::bcast(0.f);
+  // Wide rows leave few slices, so a slice may have any number of rows: their terms are added 256 at
+  // a time and the sums of those joined, in shared memory (registers are short), which keeps an fp32
+  // sum of n terms to 256 + n / 256 roundings instead of n.  A thread has slots of its own.
+  constexpr int kTogether = 256;
+  __shared__ E joined[NR * NE][kColBlock];
+#pragma unroll
+  for (int e = 0; e < NR * NE; ++e) joined[e][threadIdx.x] = M::bcast(0.f);
+  auto join = [&]() {
+#pragma unroll
+    for (int e = 0; e < NE; ++e) {
+      joined[e][threadIdx.x] = dg[e] = M::add(joined[e][threadIdx.x], dg[e]);
+      if constexpr (!RMS) joined[NE + e][threadIdx.x] = db[e] = M::add(joined[NE + e][threadIdx.x], db[e]);
+    }
+  };
   constexpr int U = 4;   // rows in flight per thread
+  int64_t next_join = r_begin + kTogether;
   for (int64_t r0 = r_begin; r0 < r_end; r0 += U) {
+    if (r0 == next_join) {
+      join();
+#pragma unroll
+      for (int e = 0; e < NE; ++e) dg[e] = db[e] = M::bcast(0.f);
+      next_join += kTogether;
+    }
     P px[U], pd[U], ps[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -186,6 +207,7 @@ __global__ void __launch_bounds__(kColBlock)
       }
     }
   }
+  join();
   float* w = a.ws + static_cast<int64_t>(blockIdx.y) * NR * a.D;
   store_param_lanes<EPV>(w, vec * EPV, dg);
   if constexpr (!RMS) store_param_lanes<EPV>(w + a.D, vec * EPV, db);

@@ -227,3 +227,26 @@ def test_heads_whose_mean_square_just_fits(lib, dtype, hd, rows, norm):
     terms = dy.double() * xh
     allow = U * (34 + 64 + 2 * rows / 16) * (dy.double().abs() * xm).sum((0, 1, 2))
     assert ((dscale.double() - terms.sum((0, 1, 2))).abs() <= allow).all()
+
+
+# ---------------------------------------------------------------------------
+# column sums of very wide rows
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("N,D", [(8192, 151553), (8192, 131080)])
+def test_column_sums_of_many_very_wide_rows(lib, N, D):
+    """Rows wider than the row-cached kernels leave few slices of rows, so a thread adds thousands of
+    terms.  Equal terms are the worst case: every addition to a growing sum rounds the same way.  Sums
+    of at most 256 terms at a time, joined one after the other, are off by 256 + N / 256 units of 2^-24
+    and a tree's 32."""
+    x = torch.ones(N, D, dtype=torch.bfloat16, device=DEV)
+    gamma = torch.ones(D, device=DEV)
+    inv = torch.full((N,), 0.1, device=DEV)
+    term = float(inv[0])
+    want, allow = N * term, U * (256 + N / 256 + 32 + 4) * N * term
+    dscale = A.fused_rms_norm_grad_op(x, x, gamma, inv)[1]
+    assert float((dscale.double() - want).abs().max()) <= allow, float((dscale.double() - want).abs().max()) / allow
+    # 1 - 0.5 = 0.5, times 0.1 rounded: exact halves of the terms above; the offset's terms are one
+    mean = torch.full((N,), 0.5, device=DEV)
+    _, dscale, doffset = A.fused_layer_norm_residual_grad_op(x, x, x, gamma, mean, inv)
+    assert float((dscale.double() - want / 2).abs().max()) <= allow / 2
+    assert float((doffset - N).abs().max()) == 0.0     # whole numbers below 2^24 are exact
