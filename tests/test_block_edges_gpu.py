@@ -230,6 +230,28 @@ def test_heads_whose_mean_square_just_fits(lib, dtype, hd, rows, norm):
 
 
 # ---------------------------------------------------------------------------
+# cosines and sines
+# ---------------------------------------------------------------------------
+def test_cosines_and_sines_keep_their_last_bit(lib):
+    """A pair (1, 0) turned by an angle is its cosine and sine.  The function on the rounded fraction of a
+    turn is off by at most one unit of 2^-24 below one (1 ulp, CUDA's bound for sinpif and cospif), the
+    correction by the part that fp32 drops rounds once more, by half a unit, and its second order,
+    (2 pi 2^-26)^2 / 2, is below 1e-14.  Without the correction the dropped part alone is up to
+    2 pi 2^-26 = 1.57 units."""
+    rows, pairs = 4096, 64
+    f = 10000.0 ** -(torch.arange(pairs, dtype=torch.float64, device=DEV) / pairs)
+    ax = torch.zeros(pairs, dtype=torch.int32, device=DEV)
+    pos = torch.randint(0, 100000, (1, rows), generator=gen(1), device=DEV)
+    q = torch.zeros(1, rows, 1, 2 * pairs, device=DEV)
+    q[..., :pairs] = 1.0
+    y = A.fused_head_norm_rotary_op(q, None, pos, f, ax, norm="none")[0][0, :, 0].double()
+    ang = pos[0, :, None].double() * f
+    # an angle's own rounding in 64 bits: 1e5 2^-53 2, in the product here and in turns there
+    err = (y - torch.cat((torch.cos(ang), torch.sin(ang)), -1)).abs()
+    assert float(err.max()) <= 1.5 * U + 1e-10, float(err.max()) / U
+
+
+# ---------------------------------------------------------------------------
 # column sums of very wide rows
 # ---------------------------------------------------------------------------
 @pytest.mark.parametrize("N,D", [(8192, 151553), (8192, 131080)])
