@@ -505,6 +505,17 @@ def instance_norm(x, gamma, beta, data_format="N...C", epsilon=0.001):
     return _instance_norm_grad.apply(x, gamma, beta, str(data_format), float(epsilon))[0]
 
 
+def _keeping_float32(fn):
+    """A module's cast (half(), to(dtype)) without the change of type: the ops take float32 parameters
+    whatever the type of the activations.  Moves to another device pass."""
+    def apply(t):
+        out = fn(t)
+        if t.dtype == torch.float32 and out.dtype != t.dtype:
+            return t.to(out.device)
+        return out
+    return apply
+
+
 # ---------------------------------------------------------------------------
 # wrapper layers
 # ---------------------------------------------------------------------------

@@ -24,8 +24,8 @@ import torch
 
 from . import _lib
 from .nv_norm_ops import (InvalidArgumentError, LayerNormalization, _axis_list, _check, _dtype_code,
-                          _first_derivatives_only, _grad_outputs, _like_output, _ln_dims, _on_device,
-                          _param, _remember, _require, fused_layer_norm_grad_op,
+                          _first_derivatives_only, _grad_outputs, _keeping_float32, _like_output, _ln_dims,
+                          _on_device, _param, _remember, _require, fused_layer_norm_grad_op,
                           fused_layer_norm_residual_op)
 
 __all__ = [
@@ -335,6 +335,9 @@ class RMSNormalization(LayerNormalization):
 
     def __init__(self, axis=-1, epsilon=1e-3, scale=True, **kwargs):
         super().__init__(axis=axis, epsilon=epsilon, center=False, scale=scale, **kwargs)
+
+    def _apply(self, fn, *args, **kwargs):
+        return super()._apply(_keeping_float32(fn), *args, **kwargs)
 
     def build(self, input_shape, device=None):
         super().build(input_shape, device=device)

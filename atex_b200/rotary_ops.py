@@ -26,8 +26,8 @@ from typing import Sequence, Tuple
 import torch
 
 from . import _lib
-from .nv_norm_ops import (InvalidArgumentError, _check, _dtype_code, _first_derivatives_only, _param, _remember,
-                          _require)
+from .nv_norm_ops import (InvalidArgumentError, _check, _dtype_code, _first_derivatives_only, _keeping_float32, _param,
+                          _remember, _require)
 from .rms_norm_ops import _on_stream, _scratch
 
 __all__ = ["fused_head_norm_rotary_op", "fused_head_norm_rotary_grad_op", "head_norm_rotary",
@@ -371,10 +371,14 @@ class HeadNormRotary(torch.nn.Module):
         self.sections, self.base, self.shared = tuple(int(s) for s in sections), float(base), bool(shared)
         self.norm, self.interleaved, self.epsilon = norm, bool(interleaved), float(epsilon)
         freq, axis = rotary_frequencies(self.sections, self.base, self.shared)
-        # plain attributes and not buffers: a module cast to half precision keeps 64-bit frequencies
+        # plain attributes and not buffers: a module cast to half precision keeps 64-bit frequencies,
+        # and its scales and offsets in 32 (_apply)
         self._rotary = (freq, axis)
         self.gamma_q = self.gamma_k = self.beta_q = self.beta_k = None
         self.built = False
+
+    def _apply(self, fn, *args, **kwargs):
+        return super()._apply(_keeping_float32(fn), *args, **kwargs)
 
     def build(self, head_dim, device=None):
         def new(value):

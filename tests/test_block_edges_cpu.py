@@ -6,6 +6,7 @@ import subprocess
 import pytest
 import torch
 
+import atex_b200 as A
 from atex_b200 import _lib as L
 from atex_b200 import rms_norm_ops as M
 
@@ -65,3 +66,29 @@ int main() {
     subprocess.run(["g++", "-std=c++17", "-I", os.path.join(ROOT, "atex_b200", "csrc"), "-I", os.path.join(cuda, "include"),
                     str(src), "-o", exe], check=True, capture_output=True, text=True)
     assert subprocess.run([exe]).returncode == 0
+
+
+# ---------------------------------------------------------------------------
+# layers cast to half precision
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("cast", [lambda m: m.half(), lambda m: m.bfloat16(), lambda m: m.to(torch.bfloat16),
+                                  lambda m: torch.nn.Sequential(m).half()[0]])
+def test_a_cast_keeps_the_layers_parameters(cast):
+    """The ops take float32 scales and offsets, also beside 16-bit activations; values, gradients and the
+    parameter objects that an optimizer holds stay."""
+    for layer, size in ((A.HeadNormRotary((4,), norm="layer"), 8), (A.RMSNormalization(), (2, 8))):
+        layer.build(size)
+        held = list(layer.parameters())
+        with torch.no_grad():
+            for i, p in enumerate(held):
+                p.uniform_(0.3, 0.7)
+                p.grad = torch.full_like(p, 1e-8 * (i + 1))   # below fp16's smallest
+        was = [(p.detach().clone(), p.grad.clone()) for p in held]
+        layer = cast(layer)
+        now = list(layer.parameters())
+        assert all(a is b for a, b in zip(held, now))
+        for p, (v, g) in zip(now, was):
+            assert p.dtype == torch.float32 and torch.equal(p, v) and torch.equal(p.grad, g)
+    layer = A.HeadNormRotary((4,))
+    layer.build(8)
+    assert layer.to("meta").gamma_q.device.type == "meta"

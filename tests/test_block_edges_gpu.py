@@ -272,3 +272,22 @@ def test_column_sums_of_many_very_wide_rows(lib, N, D):
     _, dscale, doffset = A.fused_layer_norm_residual_grad_op(x, x, x, gamma, mean, inv)
     assert float((dscale.double() - want / 2).abs().max()) <= allow / 2
     assert float((doffset - N).abs().max()) == 0.0     # whole numbers below 2^24 are exact
+
+
+# ---------------------------------------------------------------------------
+# layers cast to half precision
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("norm", ["rms", "layer", "none"])
+def test_a_cast_layer_keeps_its_parameters_in_32_bits(lib, dtype, norm):
+    q = torch.randn(1, 5, 2, 64, generator=gen(1), device=DEV).to(dtype)
+    layer = A.HeadNormRotary((16, 16), norm=norm)
+    pos = torch.arange(10, device=DEV).view(2, 5)
+    want = layer(q, q, pos)
+    layer = layer.to(dtype)
+    assert all(p.dtype == torch.float32 for p in layer.parameters())
+    got = layer(q, q, pos)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    rms = A.RMSNormalization()
+    want = rms(q)
+    assert torch.equal(rms.to(dtype)(q), want)
