@@ -48,20 +48,26 @@ _DTYPE_CODE = {torch.float32: _lib.NVN_F32, torch.float16: _lib.NVN_F16,
 
 # One scratch tensor per (device, stream), grown on demand: the analogue of the
 # OpKernelContext::allocate_temp calls in the reference functors.  Work on one
-# stream is ordered, so consecutive ops can share it.
+# stream is ordered, so consecutive ops can share it.  A captured call gets scratch of its
+# own from the graph's memory: graphs captured on one stream may be replayed on several, and
+# the shared tensor is replaced when a later call needs a larger one.
 _workspaces = {}
 
 
-def _workspace(device: torch.device, stream: int, nbytes: int) -> Tuple[int, int]:
+def _workspace(device: torch.device, stream: int, nbytes: int):
+    """(address, bytes, owner): the owner has to outlive the launch."""
     if nbytes == 0:
-        return 0, 0
+        return 0, 0, None
+    if torch.cuda.is_current_stream_capturing():
+        t = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        return t.data_ptr(), nbytes, t
     key = (device.index, stream)
     ws = _workspaces.get(key)
     if ws is None or ws[1] < nbytes:
         t = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
         ws = (t.data_ptr(), t.numel(), t)
         _workspaces[key] = ws
-    return ws[0], ws[1]
+    return ws
 
 
 # Shape bookkeeping and workspace sizes are pure functions of the problem; a training loop
@@ -245,7 +251,7 @@ def fused_layer_norm_op(x, scale, offset, axis: Iterable[int] = (-1,), epsilon: 
     with _device_guard(x.device):
         lib = _lib.load()
         stream = _stream(x.device)
-        ws_ptr, ws_bytes = _workspace(x.device, stream, _ws_bytes("nvn_ln_fwd_workspace_bytes", code, N, D))
+        ws_ptr, ws_bytes, ws_owner = _workspace(x.device, stream, _ws_bytes("nvn_ln_fwd_workspace_bytes", code, N, D))
         st = lib.nvn_ln_fwd(code, x.data_ptr(), scale.data_ptr(), offset.data_ptr(), N, D,
                             float(epsilon), y.data_ptr(), mean.data_ptr(), inv_std.data_ptr(),
                             ws_ptr, ws_bytes, stream)
@@ -283,7 +289,7 @@ def fused_layer_norm_residual_op(x, residual, scale, offset, axis: Iterable[int]
     with _device_guard(x.device):
         lib = _lib.load()
         stream = _stream(x.device)
-        ws_ptr, ws_bytes = _workspace(x.device, stream, _ws_bytes("nvn_ln_fwd_workspace_bytes", code, N, D))
+        ws_ptr, ws_bytes, ws_owner = _workspace(x.device, stream, _ws_bytes("nvn_ln_fwd_workspace_bytes", code, N, D))
         st = lib.nvn_ln_fwd_residual(code, x.data_ptr(), residual.data_ptr(), scale.data_ptr(),
                                      offset.data_ptr(), N, D, float(epsilon), s.data_ptr(),
                                      y.data_ptr(), mean.data_ptr(), inv_std.data_ptr(), ws_ptr,
@@ -342,7 +348,7 @@ def fused_layer_norm_grad_op(y_backprop, x, scale, reserve_space_1, reserve_spac
     with _device_guard(x.device):
         lib = _lib.load()
         stream = _stream(x.device)
-        ws_ptr, ws_bytes = _workspace(x.device, stream, _ws_bytes("nvn_ln_bwd_workspace_bytes", code, N, D))
+        ws_ptr, ws_bytes, ws_owner = _workspace(x.device, stream, _ws_bytes("nvn_ln_bwd_workspace_bytes", code, N, D))
         if grad_exchange is None:
             st = lib.nvn_ln_bwd(code, dy.data_ptr(), x.data_ptr(), scale.data_ptr(),
                                 mean.data_ptr(), inv_std.data_ptr(), N, D, dx.data_ptr(),
@@ -376,7 +382,7 @@ def fused_instance_norm_op(x, scale, offset, data_format: str = "N...C", epsilon
     with _device_guard(x.device):
         lib = _lib.load()
         stream = _stream(x.device)
-        ws_ptr, ws_bytes = _workspace(
+        ws_ptr, ws_bytes, ws_owner = _workspace(
             x.device, stream, _ws_bytes("nvn_in_fwd_workspace_bytes", code, N, C, D, int(cf)))
         st = lib.nvn_in_fwd(code, x.data_ptr(), scale.data_ptr(), offset.data_ptr(), N, C, D, int(cf),
                             float(epsilon), y.data_ptr(), mean.data_ptr(), inv_std.data_ptr(),
@@ -419,7 +425,7 @@ def fused_instance_norm_grad_op(y_backprop, x, scale, reserve_space_1, reserve_s
     with _device_guard(x.device):
         lib = _lib.load()
         stream = _stream(x.device)
-        ws_ptr, ws_bytes = _workspace(
+        ws_ptr, ws_bytes, ws_owner = _workspace(
             x.device, stream, _ws_bytes("nvn_in_bwd_workspace_bytes", code, N, C, D, int(cf)))
         if grad_exchange is None:
             st = lib.nvn_in_bwd(code, dy.data_ptr(), x.data_ptr(), scale.data_ptr(),

@@ -92,3 +92,25 @@ def test_a_cast_keeps_the_layers_parameters(cast):
     layer = A.HeadNormRotary((4,))
     layer.build(8)
     assert layer.to("meta").gamma_q.device.type == "meta"
+
+
+# ---------------------------------------------------------------------------
+# scratch of captured calls
+# ---------------------------------------------------------------------------
+def test_captured_calls_do_not_use_the_streams_scratch(monkeypatch):
+    """The gradient behind layer_norm_residual, like every older op, has its partial rows there.  Two graphs
+    captured on one stream may run at once, and the stream's scratch is replaced when it has to grow."""
+    from atex_b200 import nv_norm_ops as O
+    monkeypatch.setattr(O, "_workspaces", {})
+    capturing = [False]
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    device = torch.device("cpu")
+    eager = O._workspace(device, 7, 4096)
+    assert O._workspace(device, 7, 8192)[0] == eager[0]       # consecutive calls share it
+    capturing[0] = True
+    first, second = O._workspace(device, 7, 4096), O._workspace(device, 7, 4096)
+    assert len({eager[0], first[0], second[0]}) == 3
+    assert all(w[1] >= 4096 and w[2].data_ptr() == w[0] for w in (first, second))
+    assert O._workspace(device, 7, 0)[:2] == (0, 0)
+    capturing[0] = False
+    assert O._workspace(device, 7, 4096)[0] == eager[0] and len(O._workspaces) == 1

@@ -291,3 +291,41 @@ def test_a_cast_layer_keeps_its_parameters_in_32_bits(lib, dtype, norm):
     rms = A.RMSNormalization()
     want = rms(q)
     assert torch.equal(rms.to(dtype)(q), want)
+
+
+# ---------------------------------------------------------------------------
+# captured graphs of the older ops
+# ---------------------------------------------------------------------------
+def test_graphs_of_the_layer_norm_gradient_share_no_scratch(lib):
+    """Two graphs captured on one stream (torch.cuda.graph's own), replayed at once on two, and an eager call
+    that needs more scratch between capture and replay."""
+    g = gen(8)
+
+    def inputs(n):
+        x, dy = (torch.randn(n, 1024, generator=g, device=DEV).bfloat16() for _ in range(2))
+        return x, dy, torch.rand(1024, generator=g, device=DEV) + 0.5
+    problems = [inputs(3000), inputs(3000)]
+
+    def step(x, dy, w):
+        y, mean, inv = A.fused_layer_norm_op(x, w, w)
+        return (y, *A.fused_layer_norm_grad_op(dy, x, w, mean, inv))
+    want = [step(*p) for p in problems]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for p in problems:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(step(*p))
+        graphs.append(graph)
+    x = torch.randn(64, 1 << 18, generator=g, device=DEV).bfloat16()
+    w = torch.ones(1 << 18, device=DEV)
+    A.fused_layer_norm_grad_op(x, x, w, *A.fused_layer_norm_op(x, w, w)[1:])   # partial rows of 512 KB
+    streams = [torch.cuda.Stream() for _ in graphs]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(want, outs):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
