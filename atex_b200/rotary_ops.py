@@ -100,6 +100,18 @@ def _checked_out(t, like, name):
     return t
 
 
+def _own_views(outs, ins):
+    """In place means into its own input's view: into another view, or the other input, rows would be
+    written that are still to be read."""
+    for i, o in enumerate(outs):
+        for j, t in enumerate(ins):
+            if o.data_ptr() == t.data_ptr() and o.numel() and (
+                    i != j or any(a != b and n > 1 for a, b, n in zip(o.stride(), t.stride(), o.shape))):
+                raise ValueError(f"out[{i}] may share memory with its own input alone, and in the same layout")
+    if len(outs) > 1 and outs[0].data_ptr() == outs[1].data_ptr() and outs[0].numel():
+        raise ValueError("out[0] and out[1] must be different tensors")
+
+
 class _Form:
     """What the two directions need of a call's shapes, types, strides and options, once checked."""
 
@@ -254,8 +266,10 @@ def _outputs(form, q, k, out):
     q_out, k_out = out
     _checked_out(q_out, q, "out[0]")
     if k is None:
+        _own_views((q_out,), (q,))
         return q_out, None, _pack(q_out), None
     _checked_out(k_out, k, "out[1]")
+    _own_views((q_out, k_out), (q, k))
     return q_out, k_out, _pack(q_out), _pack(k_out)
 
 
@@ -278,7 +292,7 @@ def fused_head_norm_rotary_op(q, k, positions, inv_freq=None, pair_axis=None, sc
     int32 have one entry for each pair (rotary_frequencies makes them; a pair whose axis is not
     one of positions' is not rotated).  Scales and offsets are float32 of head_dim elements.
     ``out`` = (q_out, k_out) supplies the outputs as views of any layout; they may be q and k
-    themselves."""
+    themselves, and overlap nothing else that the call reads or writes."""
     form, packed, q, k, alive = _problem(q, k, positions, inv_freq, pair_axis, (scale_q, scale_k),
                                          (offset_q, offset_k), norm, interleaved, epsilon, True)
     q_out, k_out, to_q, to_k = _outputs(form, q, k, out)
@@ -295,7 +309,8 @@ def fused_head_norm_rotary_grad_op(q_backprop, k_backprop, q, k, positions, inv_
     """Gradient of fused_head_norm_rotary_op from its inputs: returns (dq, dk, dscale_q, dscale_k,
     doffset_q, doffset_k), with None for what the form does not have.  The statistics are formed
     again from q and k.  ``out`` = (dq, dk) supplies those as views of any layout, for example the
-    slices of a packed projection's gradient; they may be q_backprop and k_backprop themselves."""
+    slices of a packed projection's gradient; they may be q_backprop and k_backprop themselves, and
+    overlap nothing else that the call reads or writes."""
     form, packed, q, k, alive = _problem(q, k, positions, inv_freq, pair_axis, (scale_q, scale_k), (None, None), norm,
                                          interleaved, epsilon, False)
     _require((k is None) == (k_backprop is None), "k_backprop belongs to k")

@@ -329,3 +329,32 @@ def test_graphs_of_the_layer_norm_gradient_share_no_scratch(lib):
     torch.cuda.synchronize()
     for a, b in zip(want, outs):
         assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+# ---------------------------------------------------------------------------
+# outputs that are not their own input's view
+# ---------------------------------------------------------------------------
+def test_outputs_in_another_inputs_place_are_refused(lib):
+    g = gen(2)
+    B, T_, h, hd = 2, 6, 4, 64
+    q, k = (torch.randn(B, T_, h, hd, generator=g, device=DEV).bfloat16() for _ in range(2))
+    f, ax = A.rotary_frequencies((32,), device=DEV)
+    pos = torch.arange(T_, device=DEV)[None]
+    fresh = torch.empty_like(q)
+    other = q.view(-1).view(B, h, T_, hd).transpose(1, 2)     # q's memory, the heads in another order
+    args = (pos, f, ax)
+    for out in ((k, q), (k, fresh), (fresh, q), (fresh, fresh), (other, fresh)):
+        with pytest.raises(ValueError, match="own input|different tensors"):
+            A.fused_head_norm_rotary_op(q, k, *args, norm="none", out=out)
+        with pytest.raises(ValueError, match="own input|different tensors"):
+            A.fused_head_norm_rotary_grad_op(q, k, fresh.clone(), fresh.clone(), *args, norm="none", out=out)
+    with pytest.raises(ValueError, match="own input"):
+        A.fused_head_norm_rotary_op(q, None, *args, norm="none", out=(other, None))
+    # a size of one has no stride, and nothing at all has no address
+    one = torch.randn(1, 1, 1, hd, device=DEV)
+    want = A.fused_head_norm_rotary_op(one, None, pos[:, :1], f, ax, norm="none")[0]
+    same = one.as_strided(one.shape, (7, 9, 200, 1))
+    A.fused_head_norm_rotary_op(one, None, pos[:, :1], f, ax, norm="none", out=(same, None))
+    assert torch.equal(one, want)
+    empty = torch.empty(0, T_, h, hd, device=DEV)
+    A.fused_head_norm_rotary_op(empty, empty, *args, norm="none", out=(empty, empty))
