@@ -557,7 +557,7 @@ __global__ void __launch_bounds__(RowBlock<TPR, MINB>::kBlock)
   }
   const P* __restrict__ xp = reinterpret_cast<const P*>(a.x) + vec0;
   const P* __restrict__ dyp = reinterpret_cast<const P*>(a.dy) + vec0;
-  P* __restrict__ dxp = reinterpret_cast<P*>(a.out) + vec0;
+  P* dxp = reinterpret_cast<P*>(a.out) + vec0;   // may be a.res: not __restrict__
   const P* dsp = nullptr;
   if constexpr (DRES) dsp = reinterpret_cast<const P*>(a.res) + vec0;
 

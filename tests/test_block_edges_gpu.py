@@ -358,3 +358,24 @@ def test_outputs_in_another_inputs_place_are_refused(lib):
     assert torch.equal(one, want)
     empty = torch.empty(0, T_, h, hd, device=DEV)
     A.fused_head_norm_rotary_op(empty, empty, *args, norm="none", out=(empty, empty))
+
+
+# ---------------------------------------------------------------------------
+# gradients written over the residual branch's
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("N,D", [(300, 64), (300, 260), (300, 1001), (300, 1024), (300, 2044), (9000, 2048), (9000, 4096),
+                                 (300, 8192), (2100, 8192), (40, 16384), (40, 40000)])
+def test_a_gradient_in_the_residual_branchs_place(lib, dtype, N, D):
+    g, dt = gen(N + D), T.TORCH_DTYPE[dtype]
+    s, dy, ds = (torch.randn(N, D, generator=g, device=DEV).to(dt) for _ in range(3))
+    gamma = torch.rand(D, generator=g, device=DEV) + 0.5
+    mean, inv = torch.randn(N, generator=g, device=DEV), torch.rand(N, generator=g, device=DEV) + 0.5
+    want = A.fused_rms_norm_residual_grad_op(dy, ds, s, gamma, inv)
+    here = ds.clone()
+    got = A.fused_rms_norm_residual_grad_op(dy, here, s, gamma, inv, out=here)
+    assert got[0] is here and all(torch.equal(a, b) for a, b in zip(got, want))
+    want = A.fused_layer_norm_residual_grad_op(dy, ds, s, gamma, mean, inv)
+    here = ds.clone()
+    got = A.fused_layer_norm_residual_grad_op(dy, here, s, gamma, mean, inv, out=here)
+    assert got[0] is here and all(torch.equal(a, b) for a, b in zip(got, want))
