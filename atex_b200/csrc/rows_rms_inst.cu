@@ -48,11 +48,11 @@ cudaError_t launch_exact(const RowsResArgs& a, cudaStream_t stream, bool dry_run
   using Args = typename std::conditional<THIRD, RowsResArgs, RowsArgs>::type;
   size_t ring = 0;
   if constexpr (TMA) {
-    const size_t row_bytes = static_cast<size_t>(a.D) * sizeof(T);
-    ring = row_bytes * RPC * RB * NT * (PF >= 10 ? PF - 10 : PF);
-    if (ring > (PF >= 10 ? kMaxHeldRingBytes : kMaxRingBytes) || sizeof(Pack<T, EPV>) < 16)
-      return launch_exact<EPV, TPR, VPT, (PF >= 10 ? 1 : RB), PR, MINB, 1, EXACT, FORM>(
-          a, stream, dry_run, plan);
+    constexpr size_t kStageRows = static_cast<size_t>(RPC) * RB * NT * (PF >= 10 ? PF - 10 : PF);
+    static_assert(sizeof(Pack<T, EPV>) == 16, "ring copies move 16 bytes at least");
+    static_assert(kStageRows * TPR * VPT * EPV * sizeof(T) <= (PF >= 10 ? kMaxHeldRingBytes : kMaxRingBytes),
+                  "the ring of the widest row this shape holds must fit");
+    ring = kStageRows * static_cast<size_t>(a.D) * sizeof(T);
   }
   void (*kernel)(const Args);
   if constexpr (kBwd) {
