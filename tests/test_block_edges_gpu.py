@@ -275,6 +275,61 @@ def test_column_sums_of_many_very_wide_rows(lib, N, D):
 
 
 # ---------------------------------------------------------------------------
+# heads of zeros
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("norm", ["rms", "layer"])
+@pytest.mark.parametrize("hd,tokens", [(128, 9), (128, 2000), (96, 9), (33, 9)])
+def test_heads_of_zeros_leave_the_others_alone(lib, norm, hd, tokens):
+    """x-hat of a head of zeros is zero: it adds nothing to the scale's gradient, and its own gradient is
+    that of the others with 1/rms = 1/sqrt(eps)."""
+    g = gen(hd + tokens)
+    q = torch.randn(1, tokens, 2, hd, generator=g, device=DEV)
+    dy = torch.randn(1, tokens, 2, hd, generator=g, device=DEV)
+    q[0, ::3] = 0.0
+    scale = torch.rand(hd, generator=g, device=DEV) + 0.5
+    dx, _, dscale, _, doffset, _ = A.fused_head_norm_rotary_grad_op(dy, None, q, None, None, scale_q=scale, norm=norm,
+                                                                    epsilon=1e-6)
+    gy = dy.double() * scale.double()
+    want = (gy - gy.mean(-1, keepdim=True) if norm == "layer" else gy)[0, ::3] * 1e3
+    # 1/sqrt(1e-6) in fp32 is off by the 2^-24 of eps and 2 ulp of the root; two products and a mean
+    assert ((dx[0, ::3].double() - want).abs() <= 32 * U * (gy.abs() + gy.abs().mean(-1, keepdim=True))[0, ::3] * 1e3).all()
+    keep = torch.ones(tokens, dtype=torch.bool, device=DEV)
+    keep[::3] = False
+    x = q.double()[:, keep]
+    c = x - x.mean(-1, keepdim=True) if norm == "layer" else x
+    mag = x.abs() + x.abs().mean(-1, keepdim=True) if norm == "layer" else x.abs()
+    inv = 1 / torch.sqrt((c * c).mean(-1, keepdim=True) + 1e-6)
+    terms = dy.double()[:, keep] * c * inv
+    allow = U * (32 + 64 + 2 * tokens / 16) * (dy.double()[:, keep].abs() * mag * inv).sum((0, 1, 2))
+    assert ((dscale.double() - terms.sum((0, 1, 2))).abs() <= allow).all()
+    if norm == "layer":
+        allow = U * (32 + 64 + 2 * tokens / 16) * dy.double().abs().sum((0, 1, 2))
+        assert ((doffset.double() - dy.double().sum((0, 1, 2))).abs() <= allow).all()
+
+
+@pytest.mark.parametrize("norm", ["rms", "layer"])
+def test_heads_of_zeros_without_an_epsilon(lib, norm):
+    """0 / 0 is not a number, as in the formula: in the head's own outputs, and in the parameter sums, which
+    it is part of.  The other heads' outputs do not see it."""
+    g = gen(12)
+    q, dy = (torch.randn(1, 9, 2, 64, generator=g, device=DEV) for _ in range(2))
+    scale, off = torch.rand(64, generator=g, device=DEV) + 0.5, (torch.zeros(64, device=DEV) if norm == "layer" else None)
+    calls = []
+    for x in (q.clone(), q):
+        if x is q:
+            q[0, 4, 1] = 0.0
+        calls.append((A.fused_head_norm_rotary_op(x, None, None, scale_q=scale, offset_q=off, norm=norm, epsilon=0.0)[0],
+                      A.fused_head_norm_rotary_grad_op(dy, None, x, None, None, scale_q=scale, norm=norm, epsilon=0.0)))
+    (y0, grads0), (y, grads) = calls
+    others = torch.ones(1, 9, 2, dtype=torch.bool, device=DEV)
+    others[0, 4, 1] = False
+    assert torch.isnan(y[0, 4, 1]).all() and torch.isnan(grads[0][0, 4, 1]).all() and torch.isnan(grads[2]).all()
+    assert torch.equal(y[others], y0[others]) and torch.equal(grads[0][others], grads0[0][others])
+    if norm == "layer":
+        assert torch.equal(grads[4], grads0[4])     # the offset's sum has no 1/rms in it
+
+
+# ---------------------------------------------------------------------------
 # layers cast to half precision
 # ---------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
