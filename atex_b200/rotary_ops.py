@@ -320,6 +320,8 @@ def fused_head_norm_rotary_grad_op(q_backprop, k_backprop, q, k, positions, inv_
     if k is not None:
         k_backprop = _gradient(k_backprop, form.k_shape, q.dtype, form, "k_backprop")
     dq, dk, to_q, to_k = _outputs(form, q_backprop, k_backprop, out)
+    if out is not None and form.vectors:   # q and k are read as well
+        _own_views([t for t in (dq, dk) if t is not None], [t for t in (q, k) if t is not None])
     dparams = ws = None
     if form.vectors:
         dparams = scale_q.new_empty((form.parts * form.vectors, form.head_dim))

@@ -405,6 +405,18 @@ def test_outputs_in_another_inputs_place_are_refused(lib):
             A.fused_head_norm_rotary_grad_op(q, k, fresh.clone(), fresh.clone(), *args, norm="none", out=out)
     with pytest.raises(ValueError, match="own input"):
         A.fused_head_norm_rotary_op(q, None, *args, norm="none", out=(other, None))
+    # a gradient with a norm reads q and k too; without one it does not
+    w, dq, dk = torch.ones(hd, device=DEV), q.clone(), k.clone()
+    want = A.fused_head_norm_rotary_grad_op(dq, dk, q, k, *args, w, w)
+    for out in ((k, q), (k, fresh), (fresh, q), (other, fresh)):
+        with pytest.raises(ValueError, match="own input"):
+            A.fused_head_norm_rotary_grad_op(dq, dk, q, k, *args, w, w, out=out)
+    qq, kk = q.clone(), k.clone()
+    A.fused_head_norm_rotary_grad_op(dq, dk, qq, kk, *args, w, w, out=(qq, kk))
+    assert torch.equal(qq, want[0]) and torch.equal(kk, want[1])
+    want = A.fused_head_norm_rotary_grad_op(dq, dk, q, k, *args, norm="none")
+    got = A.fused_head_norm_rotary_grad_op(dq, dk, q, k, *args, norm="none", out=(k, q))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     # a size of one has no stride, and nothing at all has no address
     one = torch.randn(1, 1, 1, hd, device=DEV)
     want = A.fused_head_norm_rotary_op(one, None, pos[:, :1], f, ax, norm="none")[0]
