@@ -11,9 +11,9 @@
 //   place of two more tensors.
 //
 // Both directions move 2 (forward) or 3 (gradient) passes over q and k and are bound by HBM when
-// there are rows enough: bf16, 32+8 packed heads of 128, 32768 tokens forward 111 us (6.1 TB/s, 93 % of
-// the measured copy rate), 16384 tokens gradient 88 us (5.7 TB/s).  What stands between that and the
-// copy rate is a row's dependent chain (unpack, sums, shuffles, rotation) on 16 to 20 warps an SM.
+// there are rows enough: bf16, 32+8 packed heads of 128, 32768 tokens forward 116 us (5.8 TB/s, 89 % of
+// the measured copy rate), 16384 tokens gradient 91 us (5.6 TB/s, 85 %).  What stands between that and
+// the copy rate is a row's dependent chain (unpack, sums, shuffles, rotation) on 16 to 20 warps an SM.
 //
 // Layout.  A head is a row of head_dim elements; TPH lanes of a warp (a power of two) own it, 16
 // elements each, as SPT slots of two vectors (A, B) of V elements:
@@ -28,7 +28,9 @@
 // a token has more rows than a tile, or tokens are few, a piece of the block's rows.  The angles of a
 // token are the same for all its heads and are computed once per tile into shared memory - in 64
 // bits up to the fraction of a turn, because a position of a million times a frequency has no
-// fraction left in 32.  Where each row of a tile begins is worked out once as well, by one thread a
+// fraction left in 32; cosine and sine are fp32 functions of the fraction rounded to fp32, corrected
+// by what the rounding dropped (1.3 units of 2^-24 at worst, measured; a rounded 64-bit value has
+// 0.5).  Where each row of a tile begins is worked out once as well, by one thread a
 // row (done by every lane for every row it was a fifth of the instructions).  The rows of a tile
 // are dealt to the groups of TPH lanes; while a group works on a row its next one is already on the
 // way into registers, across the ends of parts and tiles too.  The tables (angles, row addresses)
@@ -594,7 +596,9 @@ __global__ void __launch_bounds__(head_block(R), head_ctas(BWD, R, NORM, PAD)) h
         if constexpr (NORM != 0) {
           // sum of squares; backward: sum gy c and, for mean and variance, sum gy beside it
           constexpr int NR = BWD ? NORM + 1 : 1;
-          // squares scaled down by a power of two, as many as a lane adds at once: see rows_fwd_kernel
+          // squares scaled down by a power of two, as many as a lane adds at once: see rows_fwd_kernel.
+          // (Up to 3 % for heads bound by instructions.  Adding again only where a sum overflowed
+          // costs the gradient registers: bf16 16384 tokens 91 -> 109 us.)
           constexpr float kSquares = kSquaresOverflow<T> ? 2 * V : 1;
           const E down = M::bcast(1.f / kSquares);
           float red[NR * R];
@@ -619,7 +623,7 @@ __global__ void __launch_bounds__(head_block(R), head_ctas(BWD, R, NORM, PAD)) h
                   }
                 }
 #pragma unroll
-              for (int k = 0; k < NR; ++k)   // shares of means: no overflow in the sum
+              for (int k = 0; k < NR; ++k)   // shares of means: no overflow in the sum over the lanes
                 if (ok[i]) red[r * NR + k] += M::hsum(acc[k]) * (k == 0 ? a.inv_hd * kSquares : a.inv_hd);
             }
           }

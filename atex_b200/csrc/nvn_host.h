@@ -311,7 +311,7 @@ cudaError_t residual_add_launch(int dtype, const void* x, const void* res, void*
 // against the LayerNorm tables' shape of the same width:
 //   forward: small CTAs that keep the next row in registers beat the rings, whose barriers the
 //     one reduction does not hide (bf16 [32768, 4096] plain 97 -> 84 us, residual 181 -> 170 us,
-//     where 192 threads, 21 of them with a vector less, beat 128 that fit); wide rows of the residual
+//     where 192 threads, 64 of them with a vector less, beat 128 that fit); wide rows of the residual
 //     form load on demand ([16384, 8192] 186 -> 166 us, [4096, 32768] 219 -> 177 us).
 //   backward: two stages and a warp or two per row (f16 [65536, 1024] LayerNorm 93 -> 85 us, bf16
 //     [32768, 2048] RMS residual 107 -> 84 us).  Where three tensors are read, two rows at once and

@@ -14,7 +14,8 @@ scale and offset) or ``"none"`` - and its pair p is turned by the angle
 ``positions[pair_axis[p], batch, token] * inv_freq[p]``.  The axes may be time, height and width
 of a video, row and column of an image, or the one of a text.  Pair p is the elements
 (p, p + pairs), or (2p, 2p + 1) with ``interleaved``; elements from 2 * pairs on are not rotated.
-Angles are formed in 64 bits, everything else in float32, rounded once to the type of q and k.
+Angles are formed in 64 bits up to the fraction of a turn; cosine and sine (off by at most 1.5
+units of 2^-24) and everything else are float32, rounded once to the type of q and k.
 A head of zeros has x-hat 0, unless epsilon is 0 as well: then it is 0 / 0 and NaN, in its own
 outputs and in the parameter sums.
 

@@ -207,8 +207,9 @@ NVN_API int nvn_rms_bwd(int dtype, const void* dy, const void* dsum, const void*
  *   pair p turns by angle = position[pair_axis[p], batch, token] inv_freq[p]:
  *   (u, v) -> (u cos - v sin, u sin + v cos)
  * Pair p is the elements (p, p + pairs) of a head, or (2p, 2p + 1) when `interleaved`; elements
- * from 2 pairs on are normalised and not rotated.  Angles are formed in 64 bits, everything
- * else in fp32, with one rounding to T.  A pair whose axis is not in [0, axes) is not rotated.
+ * from 2 pairs on are normalised and not rotated.  Angles are formed in 64 bits up to the
+ * fraction of a turn; cosine and sine (off by at most 1.5 units of 2^-24) and everything else are
+ * fp32, with one rounding to T.  A pair whose axis is not in [0, axes) is not rotated.
  *   - nvn_heads: a view.  The elements of a head are contiguous, the three strides (in
  *     elements) are free: a slice of a packed projection, head-major tensors and so on.  An
  *     output may be the input's own view (in place); otherwise outputs overlap nothing.
