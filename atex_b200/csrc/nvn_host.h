@@ -343,7 +343,9 @@ constexpr int64_t kRmsHeldMinBytes = 32ll << 20;
 // Accesses of less than 128 bits.  Against the LayerNorm table: f16 [12345, 1001] 20.3 -> 12.5 us
 // forward, 58 -> 34 us LayerNorm backward; bf16 [29363, 2347] residual 258 -> 122 us.  The widest
 // entry holds 16 values of four tensors per thread, too many with the dbeta sums (f16 [4000, 7031]
-// LayerNorm 152 us, 106 us by the kernels for any width).
+// LayerNorm 152 us, 106 us by the kernels for any width).  Those figures are of single elements; 16-bit
+// widths that four divides and eight does not hold four times the values in the same entries, and their
+// gradients spill (0.2 to 4.8 KB a thread).
 #define NVN_RMS_NARROW_SHAPES(X)                                                               \
   X(0, 8, 4, 2, 128, 1, 7)    X(1, 32, 4, 4, 128, 1, 7)   X(2, 32, 8, 2, 128, 1, 7)             \
   X(3, 32, 16, 1, 128, 1, 7)  X(4, 64, 16, 1, 128, 1, 7)  X(5, 128, 16, 1, 128, 1, 7)           \
